@@ -62,6 +62,20 @@ class Stats(C.Structure):
                 ("weight_bytes", C.c_uint64), ("kv_bytes", C.c_uint64), ("last_step_us", C.c_double)]
 
 
+class PagedCacheDesc(C.Structure):
+    _fields_ = [("k", _p), ("v", _p), ("block_table", _p), ("lengths", _p), ("weights", _p),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("table_stride", C.c_int64), ("type", C.c_int32), ("seqs", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32), ("max_pages", C.c_int32),
+                ("pad_", C.c_int32)]
+
+
+class PagedAttn(C.Structure):
+    _fields_ = [("q", _p), ("o", _p), ("q_row", C.c_int64), ("q_head", C.c_int64), ("o_row", C.c_int64),
+                ("o_head", C.c_int64), ("sinks", _p), ("scale", C.c_float), ("heads", C.c_int32),
+                ("window", C.c_int32), ("first", C.c_int32)]
+
+
 class HcError(RuntimeError):
     """An error string returned by the library."""
 
@@ -124,6 +138,15 @@ SIGNATURES = {
     "hc_argmax_run": (_err, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
     "hc_route_run": (_err, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
                             C.c_void_p]),
+    "hc_paged_append_run": (_err, [_p, _p, _p, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _p, _p, C.c_int32, _p]),
+    "hc_paged_decode_run": (_err, [_p, _p, C.c_int32, C.c_int32, _p, C.c_uint64, _p]),
+    "hc_paged_decode_scratch": (_err, [_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                       C.POINTER(C.c_uint64)]),
+    "hc_paged_prompt_run": (_err, [_p, _p, _p, C.c_int32, C.c_int32, C.c_int32, _p, C.c_uint64, _p]),
+    "hc_paged_prompt_scratch": (_err, [_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                       C.POINTER(C.c_uint64)]),
+    "hc_paged_evict_run": (_err, [_p, _p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _p, _p, C.c_uint64, _p]),
+    "hc_paged_evict_scratch": (_err, [_p, C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
 }
 
 _HERE = os.path.dirname(os.path.abspath(__file__))

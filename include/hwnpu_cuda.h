@@ -398,6 +398,105 @@ HC_API char *hc_argmax_run(const uint16_t *logits, int32_t rows, int32_t vocab, 
 HC_API char *hc_route_run(const float *logits, int32_t rows, int32_t n, int32_t k, int32_t *idx,
                           float *w, void *stream);
 
+/* ---------------------------------------------------------------------------------------- */
+/* Attention over a caller's paged 16-bit cache                                              */
+/* (pointers are device addresses; stream is a cudaStream_t or NULL for the default stream)   */
+/* ---------------------------------------------------------------------------------------- */
+
+/* A key-value cache in pages, owned by the caller: the long-context counterpart of the engine's own
+ * caches (the reference keeps a long conversation in pages too, internal/llm/paged.go:227-310, and
+ * its sliding layers in a ring, gptoss/build.go:291-326). Slot j of sequence i is row j % page_size of
+ * page block_table[i][j / page_size]; row r of head h of page p starts p * page_stride +
+ * h * head_stride + r * row_stride elements behind k (and v), its head_dim elements contiguous.
+ *
+ * Every call only enqueues work on stream: nothing is allocated, copied to the host or waited for, so
+ * calls can be captured in a CUDA graph and replayed with other lengths. Errors of the arguments and
+ * of the launches are returned, errors of the execution show on the stream. The descriptor may be
+ * freed when the call returns.
+ *
+ * lengths, block_table and the row lists below are device memory and are not checked by the host. The
+ * kernels hold them to their ranges: a length below 0 counts as 0 and one above max_pages * page_size
+ * as that; a page id outside [0, pages) reads as a page of zeros and is never written. */
+typedef struct hc_paged_cache {
+  void *k, *v;                 /* fp16 or bf16, 16-byte aligned */
+  const int32_t *block_table;  /* [seqs][table_stride], the first max_pages of each row */
+  int32_t *lengths;            /* [seqs]: slots in use */
+  float *weights;              /* [seqs][kv_heads][max_pages * page_size] accumulated attention
+                                * weights, or NULL */
+  int64_t page_stride, head_stride, row_stride; /* elements, multiples of 8 */
+  int64_t table_stride;        /* entries */
+  int32_t type;                /* HC_FMT_F16 or HC_FMT_BF16 */
+  int32_t seqs, kv_heads;
+  int32_t head_dim;            /* 64 or 128 */
+  int32_t page_size;           /* a power of two, 16..1024 */
+  int32_t pages;               /* pages k and v hold */
+  int32_t max_pages;           /* most pages of a sequence; max_pages * page_size < 2^30 */
+  int32_t pad_;
+} hc_paged_cache;
+
+/* The query side of an attention call. A query at slot p sees the slots j <= p with
+ * p - j < window (window 0: all of them) or j < first: a sliding window behind a few first tokens that
+ * stay visible. o = sum_j w_j v_j with w_j = exp(s_j) / (sum_j exp(s_j) + exp(sinks[head])),
+ * s_j = scale * q . k_j (blocks.SDPAGrouped blocks.go:516-539; the sink logit of gpt-oss's sdpaSink,
+ * gptoss/build.go:256-285, without sinks that term is absent). A query that sees nothing writes
+ * zeros. Slots that no query sees may hold anything, infinities and NaN included; in
+ * hc_paged_prompt_run a value row that one query sees and another of the same call does not has to
+ * be finite. */
+typedef struct hc_paged_attn {
+  const void *q;               /* [rows][heads][head_dim] of the cache's type, 16-byte aligned */
+  void *o;                     /* [rows][heads][head_dim] of the cache's type, 16-byte aligned */
+  int64_t q_row, q_head, o_row, o_head; /* strides in elements, multiples of 8 */
+  const float *sinks;          /* [heads], or NULL */
+  float scale;
+  int32_t heads;               /* a multiple of kv_heads: query head h reads kv head
+                                * h / (heads / kv_heads) */
+  int32_t window, first;
+} hc_paged_attn;
+
+/* Writes `rows` new rows into the pages (Session.Step's key-value write, decode.go:1668-1705): row r of k
+ * and v ([rows][kv_heads][head_dim], strides in elements, multiples of 8) into slot slot[r] of
+ * sequence seq[r], both int32 device arrays; the slot's accumulated weight becomes 0 when the cache
+ * has weights. A row whose sequence, slot or page is out of range (a negative slot marks padding) is
+ * left out. Lengths are the caller's to move. Two rows of a call with the same slot leave either. */
+HC_API char *hc_paged_append_run(const hc_paged_cache *c, const void *k, const void *v, int64_t k_row,
+                                 int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *seq,
+                                 const int32_t *slot, int32_t rows, void *stream);
+
+/* Attention of one new token a sequence, q row i being the token in slot lengths[i] - 1 of sequence
+ * i, split over the cache's length and joined (Flash-Decoding's merge, paged.go:227-310). max_len is the
+ * caller's bound of the lengths, for the split alone (0: the capacity); a longer sequence is
+ * still read whole. With accumulate != 0 the cache's weights of every visible slot grow by the sum of
+ * w_j over the kv head's query heads. scratch: hc_paged_decode_scratch bytes, 16-byte aligned, its
+ * contents arbitrary and not kept; calls that overlap in time need scratch of their own. */
+HC_API char *hc_paged_decode_run(const hc_paged_cache *c, const hc_paged_attn *a, int32_t max_len,
+                                 int32_t accumulate, void *scratch, uint64_t scratch_bytes, void *stream);
+HC_API char *hc_paged_decode_scratch(const hc_paged_cache *c, int32_t heads, int32_t window, int32_t first,
+                                     int32_t max_len, int32_t accumulate, uint64_t *bytes);
+
+/* Attention of many new tokens a sequence, whose keys and values are in the pages already: q rows
+ * starts[i] .. starts[i + 1] - 1 (int32 device array [seqs + 1], not decreasing, starts[0] = 0,
+ * starts[seqs] = rows) are the last slots of sequence i, in order. max_rows is the caller's bound of a
+ * sequence's rows: rows past it are not written. max_len and scratch as in hc_paged_decode_run. */
+HC_API char *hc_paged_prompt_run(const hc_paged_cache *c, const hc_paged_attn *a, const int32_t *starts,
+                                 int32_t rows, int32_t max_rows, int32_t max_len, void *scratch,
+                                 uint64_t scratch_bytes, void *stream);
+HC_API char *hc_paged_prompt_scratch(const hc_paged_cache *c, int32_t heads, int32_t window, int32_t first,
+                                     int32_t rows, int32_t max_rows, int32_t max_len, uint64_t *bytes);
+
+/* Cuts every sequence to at most `keep` slots a head and copies them, in slot order, into the pages of
+ * `to`: its first `first` slots, its last `recent`, and of those between the ones with the largest
+ * accumulated weights (of two equal ones the lower slot; NaN counts below every number). Sequences of
+ * at most keep slots are copied whole. Each kv head keeps slots of its own. to->lengths and, when `to`
+ * has them, to->weights are written; kept (int32 [seqs][kv_heads][keep], or NULL) gets the slots the rows
+ * came from, -1 past the new length. `to` has the type, heads, head_dim and seqs of c, may share its
+ * pools and page size or have others, and none of its pages may be one that c's sequences use: pages
+ * that other sequences share stay as they are, and the caller frees the old ones. scratch:
+ * hc_paged_evict_scratch bytes, as in hc_paged_decode_run. */
+HC_API char *hc_paged_evict_run(const hc_paged_cache *c, const hc_paged_cache *to, int32_t keep, int32_t first,
+                                int32_t recent, int32_t max_len, int32_t *kept, void *scratch,
+                                uint64_t scratch_bytes, void *stream);
+HC_API char *hc_paged_evict_scratch(const hc_paged_cache *c, int32_t keep, int32_t max_len, uint64_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif
