@@ -1,108 +1,496 @@
 // paged_decode.cu: attention of one new token a sequence over a caller's paged 16-bit cache
-// (hc_paged_decode_run), and of many new tokens (hc_paged_prompt_run).
+// (hc_paged_decode_run): softmax(scale q K^T) V over the visible slots, the cache's length split over
+// CTAs and joined (Flash-Decoding, paged.go:227-310).
+//
+// Bound. A visible slot costs 4 head_dim bytes of HBM (its key and its value, once for all the query
+// heads of the kv head) and 4 head_dim flops a query head: at most 8 flops a byte with 8 heads, far
+// below the card's balance, so the kernel is bound by HBM and everything else only has to stay out of
+// the loads' way.
+//
+// Split. One CTA a (range of slots, kv head, sequence), 4 warps. The visible slots are taken in groups of 16
+// aligned ones (a group never leaves its page: pages have 16 << n slots): first the groups of the
+// first tokens that stay visible, then those of the window. A warp takes every fourth group of the
+// CTA's range through its own shared-memory ring (cp.async, 16 bytes a lane, no barrier between the
+// warps), so that 2 or 3 groups a warp are always in flight. Slots of an edge group that the mask
+// hides are filled with zeros instead of being read.
+//
+// Arithmetic, a group at a time, up to 8 query heads (more take further CTAs, which find the rows in
+// the L2 cache):
+//   S = Q K^T    mma.sync m16n8k16, rows 0-7 of A the heads, B the key rows by ldmatrix
+//   P            exp2(S - m) in float32 with the running maximum m and sum l of each head. m is only
+//                moved when a score passes it by more than 2^8 (then O and l are rescaled), which is
+//                exact either way: P stays at most 256
+//   O += P V     the same MMA: rows 0-7 of A are P rounded to the cache's type, rows 8-15 what the
+//                rounding left of P (rounded in its turn), so that the weights carry 16 bits or more
+//                at no further MMA; B is V by ldmatrix.trans. O is float32
+// The four warps' (m, l, O) are joined in shared memory, the splits' by a second kernel, both in a
+// fixed order. With `accumulate` the scores are kept in scratch (float32) and the visible slots' weights
+// exp2(S - m) / l are summed over the heads once m and l are known.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "device.cuh"
+#include "kernels.h"
 #include "paged.h"
 
 namespace hc {
 namespace {
 
-__device__ __forceinline__ float paged_val(uint16_t b, bool bf16) {
-  return bf16 ? __uint_as_float(uint32_t(b) << 16) : __half2float(__ushort_as_half(b));
+constexpr int kPdWarps = 4;
+constexpr int kPdGroup = 16;   // slots of a group
+constexpr int kPdHeads = 8;    // query heads a CTA
+constexpr float kPdLazy = 8.f;  // log2 of how far a score may pass the running maximum
+constexpr float kPdLog2e = 1.4426950408889634f;
+
+template <int HD>
+struct PdRing {
+  static constexpr int kRow = HD * 2;             // bytes of a row
+  static constexpr int kHalf = kPdGroup * kRow;   // keys (or values) of a group
+  static constexpr int kStage = 2 * kHalf;
+  // groups a warp keeps in shared memory: 96 KB (128) or 64 KB (64) a CTA, two or three CTAs an SM,
+  // 128 to 144 KB in flight on an SM
+  static constexpr int kStages = HD == 128 ? 3 : 4;
+  static constexpr int kBytes = kPdWarps * kStages * kStage;
+  __device__ static __forceinline__ int off(int r, int ch) { return r * kRow + ((ch ^ (r & 7)) << 4); }
+};
+
+__device__ __forceinline__ uint32_t pd_saddr(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-__device__ __forceinline__ uint16_t paged_bits(float v, bool bf16) {
-  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+// 16 bytes to shared memory, or 16 zero bytes (nothing is read) when !there.
+__device__ __forceinline__ void pd_cp16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pd_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pd_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <bool TRANS>
+__device__ __forceinline__ void pd_ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  if (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ void pd_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  if (BF)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// a in the low half, b in the high half, rounded to nearest even.
+template <bool BF>
+__device__ __forceinline__ uint32_t pd_pack(float a, float b) {
+  if (BF) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&x);
+  }
+  const __half2 x = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&x);
+}
+template <bool BF>
+__device__ __forceinline__ float2 pd_unpack(uint32_t v) {
+  if (BF) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
-// One CTA a (row, kv head), a warp a query head at a time: the lanes share a key's dimensions, the
-// softmax runs with its maximum and sum.
-template <int HD>
-__global__ void __launch_bounds__(256) paged_rows_kernel(PagedView c, PagedQuery a, const int32_t *__restrict__ starts,
-                                                         int rows, int max_rows, bool accumulate) {
-  constexpr int E = HD / 32;
-  __shared__ float sm_m[128], sm_l[128];
-  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int i = blockIdx.z, row = i, n = paged_len(c, i), p = n - 1;
-  if (starts) {
-    const int t = blockIdx.x;
-    row = starts[i] + t;
-    const int cnt = starts[i + 1] - starts[i];
-    if (t >= cnt || t >= max_rows || row < 0 || row >= rows) return;
-    p = n - cnt + t;
+// The visible slots of a query at slot n - 1 as groups of 16: ga of them from slot 0 on, then gb from slot
+// 16 b0 on; slot j of them is seen when j < n and (j >= lo or j < first).
+struct PdSpan {
+  int n, lo, first, ga, b0, groups;
+  __device__ __forceinline__ PdSpan(int len, int window, int first_) : n(len), first(first_) {
+    lo = window > 0 && n > window ? n - window : 0;
+    first = min(first_, lo);
+    ga = (first + kPdGroup - 1) / kPdGroup;
+    b0 = max(lo / kPdGroup, ga);
+    groups = n > 0 ? ga + max(0, (n + kPdGroup - 1) / kPdGroup - b0) : 0;
   }
-  auto score = [&](const float (&q)[E], int64_t at) {
-    float s = 0.f;
-    if (at >= 0)
-#pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(q[e], paged_val(c.k[at + lane + 32 * e], c.bf16), s);
-    return warp_sum(s) * a.scale;
+  __device__ __forceinline__ int slot(int g) const { return (g < ga ? g : g - ga + b0) * kPdGroup; }
+  __device__ __forceinline__ bool sees(int j) const { return j < n && (j >= lo || j < first); }
+  // groups of one split when the work is cut in up to `splits`
+  __device__ __forceinline__ int per(int splits) const {
+    return max(1, (groups + splits * kPdWarps - 1) / (splits * kPdWarps)) * kPdWarps;
+  }
+};
+
+struct PdArgs {
+  PagedView c;
+  PagedQuery a;
+  int splits, hgroups;
+  bool accumulate;
+  int64_t score_stride;  // scores a head keeps in scratch
+  float *part_ml;        // [seqs][heads][splits][2]: m (log2 units) and l
+  float *part_o;         // [seqs][heads][splits][hd], not divided by l
+  float *scores;         // [seqs][heads][score_stride], log2 units, by group
+};
+
+// The weights of groups [g0, g1) of (sequence i, kv head h), once each head's m and 1 / l are in ml.
+__device__ __forceinline__ void pd_add_weights(const PdArgs &p, const PdSpan &sp, int i, int h, int g0, int g1,
+                                               const float2 *ml) {
+  float *w = p.c.weights + (int64_t(i) * p.c.kv_heads + h) * p.c.cap;
+  const float *s0 = p.scores + (int64_t(i) * p.a.heads + int64_t(h) * p.a.rep) * p.score_stride;
+  for (int u = g0 * kPdGroup + threadIdx.x; u < g1 * kPdGroup; u += blockDim.x) {
+    const int j = sp.slot(u / kPdGroup) + u % kPdGroup;
+    if (!sp.sees(j)) continue;
+    float add = 0.f;
+    for (int r = 0; r < p.a.rep; ++r) add += exp2f(s0[r * p.score_stride + u] - ml[r].x) * ml[r].y;
+    w[j] += add;
+  }
+}
+
+template <int HD, bool BF>
+__global__ void __launch_bounds__(kPdWarps * 32, HD == 128 ? 2 : 3) paged_decode_kernel(const PdArgs p) {
+  using Ring = PdRing<HD>;
+  constexpr int KS = HD / 16;  // k-steps of S = Q K^T
+  constexpr int NT = HD / 8;   // column tiles of O
+  constexpr int CH = HD / 8;   // 16-byte pieces of a row
+  constexpr int RPS = 32 / CH;  // rows a warp copies an instruction
+  // P is held 2^kBias above exp2(S - m): fp16's smallest weights, 2^-25, then stand for 2^-32, and its
+  // largest for 2^15
+  constexpr float kBias = BF ? 0.f : 7.f;
+  extern __shared__ __align__(128) uint8_t pd_buf[];
+  __shared__ float sm_m[kPdWarps][kPdHeads], sm_l[kPdWarps][kPdHeads];
+  __shared__ float2 sm_ml[kPdHeads];
+  pdl_trigger();
+  pdl_wait();
+  const PagedView &c = p.c;
+  const int split = blockIdx.x, h = blockIdx.y / p.hgroups, hg = blockIdx.y % p.hgroups, i = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, cq = lane & 3;
+  const PdSpan sp(paged_len(c, i), p.a.window, p.a.first);
+  const int per = sp.per(p.splits);
+  const int g0 = split * per, g1 = min(sp.groups, g0 + per);
+  if (g0 >= g1 && split > 0) return;
+  const bool alone = sp.groups <= per;  // this CTA has the whole row
+  const int head0 = h * p.a.rep + hg * kPdHeads, nheads = min(kPdHeads, p.a.rep - hg * kPdHeads);
+
+  // the warp's page ids: lane k has that of its k-th group from `at` on, the next 32 are on their way
+  const int32_t *table = c.table + i * c.table_stride;
+  auto page_of = [&](int k) {
+    const int g = g0 + warp + k * kPdWarps;
+    return g < g1 ? table[sp.slot(g) >> c.shift] : -1;
   };
-  auto sees = [&](int j) { return a.window == 0 || p - j < a.window || j < a.first; };
-  for (int r = warp; r < a.rep; r += 8) {
-    const int hq = h * a.rep + r;
-    float q[E], o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      q[e] = paged_val(a.q[row * a.q_row + hq * a.q_head + lane + 32 * e], c.bf16);
-      o[e] = 0.f;
+  int ids_cur = page_of(lane), ids_nxt = page_of(32 + lane);
+  uint8_t *ring = pd_buf + warp * Ring::kStages * Ring::kStage;
+  const uint32_t ring_s = pd_saddr(ring);
+  const int row0 = lane / CH, ch = lane % CH;
+  const int64_t head_off = h * c.head_stride;
+  // group k of the warp into its ring; k only grows
+  auto issue = [&](int k) {
+    const int g = g0 + warp + k * kPdWarps;
+    if (k && (k & 31) == 0) {
+      ids_cur = ids_nxt;
+      ids_nxt = page_of(k + 32 + lane);
     }
-    float m = a.sinks ? a.sinks[hq] : -INFINITY, l = a.sinks ? 1.f : 0.f;
-    if (m == -INFINITY) l = 0.f;
-    for (int j = 0; j <= p; ++j) {
-      if (!sees(j)) continue;
-      const int64_t at = paged_row(c, i, h, j);
-      const float s = score(q, at);
-      const float nm = fmaxf(m, s);
-      const float f = m == -INFINITY ? 0.f : expf(m - nm), w = nm == -INFINITY ? 0.f : expf(s - nm);
-      l = l * f + w;
+    const int page = __shfl_sync(0xffffffffu, ids_cur, k & 31);
+    if (g < g1) {
+      const int j0 = sp.slot(g);
+      const bool in_pool = unsigned(page) < unsigned(c.pages);
+      const bool whole = in_pool && j0 + kPdGroup <= sp.n && (j0 >= sp.lo || j0 + kPdGroup <= sp.first);
+      const int64_t at = (in_pool ? page : 0) * c.page_stride + head_off +
+                         int64_t((j0 & ((1 << c.shift) - 1)) + row0) * c.row_stride + ch * 8;
+      const uint16_t *ks = c.k + at, *vs = c.v + at;
+      const uint32_t dst = ring_s + (k % Ring::kStages) * Ring::kStage;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * f + (at >= 0 ? w * paged_val(c.v[at + lane + 32 * e], c.bf16) : 0.f);
+      for (int s = 0; s < kPdGroup / RPS; ++s) {
+        const int r = row0 + s * RPS;
+        const bool there = whole || (in_pool && sp.sees(j0 + r));
+        pd_cp16(dst + Ring::off(r, ch), ks + s * RPS * c.row_stride, there);
+        pd_cp16(dst + Ring::kHalf + Ring::off(r, ch), vs + s * RPS * c.row_stride, there);
+      }
+    }
+    pd_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < Ring::kStages - 1; ++k) issue(k);
+
+  // the query heads as A fragments (rows 8-15 are zero)
+  uint32_t qa[KS][2];
+  {
+    const uint16_t *q = p.a.q + i * p.a.q_row + (head0 + gq) * p.a.q_head + 2 * cq;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qa[s][0] = gq < nheads ? *reinterpret_cast<const uint32_t *>(q + 16 * s) : 0u;
+      qa[s][1] = gq < nheads ? *reinterpret_cast<const uint32_t *>(q + 16 * s + 8) : 0u;
+    }
+  }
+  const float scale2 = p.a.scale * kPdLog2e;  // scores in log2 units
+  float m = -INFINITY, l = 0.f;                          // of head gq, the same on its 4 lanes (l: this lane's part)
+  float o[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+  float *score_row = p.accumulate && gq < nheads ? p.scores + (int64_t(i) * p.a.heads + head0 + gq) * p.score_stride : nullptr;
+  const int lm = lane >> 3, lr = lane & 7;
+
+  for (int k = 0; g0 + warp + k * kPdWarps < g1; ++k) {
+    const int g = g0 + warp + k * kPdWarps;
+    issue(k + Ring::kStages - 1);
+    pd_wait<Ring::kStages - 1>();
+    __syncwarp();
+    const uint32_t buf = ring_s + (k % Ring::kStages) * Ring::kStage;
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};  // slots 0-7 and 8-15
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint32_t b[4];
+      pd_ldsm4<false>(buf + Ring::off((lm >> 1) * 8 + lr, 2 * s + (lm & 1)), b);
+      pd_mma<BF>(s0, qa[s][0], 0u, qa[s][1], 0u, b[0], b[1]);
+      pd_mma<BF>(s1, qa[s][0], 0u, qa[s][1], 0u, b[2], b[3]);
+    }
+    const int j0 = sp.slot(g);
+    float x[4] = {s0[0] * scale2, s0[1] * scale2, s1[0] * scale2, s1[1] * scale2};  // slots 2c, 2c+1, 8+2c, 9+2c
+    if (!(j0 + kPdGroup <= sp.n && (j0 >= sp.lo || j0 + kPdGroup <= sp.first))) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!sp.sees(j0 + 2 * cq + (e & 1) + 8 * (e >> 1))) x[e] = -INFINITY;
+    }
+    if (score_row) {
+      *reinterpret_cast<float2 *>(score_row + g * kPdGroup + 2 * cq) = make_float2(x[0], x[1]);
+      *reinterpret_cast<float2 *>(score_row + g * kPdGroup + 8 + 2 * cq) = make_float2(x[2], x[3]);
+    }
+    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if (__any_sync(0xffffffffu, mx > m + kPdLazy || (m == -INFINITY && mx > m))) {
+      const float nm = fmaxf(m, mx);
+      const float f = m == -INFINITY ? 0.f : exp2f(m - nm);
       m = nm;
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+      l *= f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) a.o[row * a.o_row + hq * a.o_head + lane + 32 * e] = paged_bits(o[e] * inv, c.bf16);
-    if (lane == 0) {
-      sm_m[r] = m;
-      sm_l[r] = inv;
+      for (int t = 0; t < NT; ++t) {
+        // rows 0-7 and what their rounding left, rows 8-15, belong to one head
+        o[t][0] *= f;
+        o[t][1] *= f;
+        o[t][2] *= f;
+        o[t][3] *= f;
+      }
     }
+    const float ref = m == -INFINITY ? 0.f : m - kBias;
+    float e[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      e[y] = exp2f(x[y] - ref);
+      l += e[y];
+    }
+    const uint32_t p0 = pd_pack<BF>(e[0], e[1]), p1 = pd_pack<BF>(e[2], e[3]);
+    const float2 h0 = pd_unpack<BF>(p0), h1 = pd_unpack<BF>(p1);
+    const uint32_t r0 = pd_pack<BF>(e[0] - h0.x, e[1] - h0.y), r1 = pd_pack<BF>(e[2] - h1.x, e[3] - h1.y);
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      uint32_t b[4];
+      pd_ldsm4<true>(buf + Ring::kHalf + Ring::off((lm & 1) * 8 + lr, t + (lm >> 1)), b);
+      pd_mma<BF>(o[t], p0, r0, p1, r1, b[0], b[1]);
+      pd_mma<BF>(o[t + 1], p0, r0, p1, r1, b[2], b[3]);
+    }
+    __syncwarp();  // the stage is read before it is filled again
   }
-  if (!accumulate) return;
+  pd_wait<0>();
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  __syncthreads();  // every warp is done with its ring
+
+  // join the warps: [warp][head][hd] float32 in the ring's memory
+  float *po = reinterpret_cast<float *>(pd_buf);
+  if (cq == 0) {
+    sm_m[warp][gq] = m - kBias;
+    sm_l[warp][gq] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    *reinterpret_cast<float2 *>(po + (warp * kPdHeads + gq) * HD + 8 * t + 2 * cq) =
+        make_float2(o[t][0] + o[t][2], o[t][1] + o[t][3]);
   __syncthreads();
-  for (int j = warp; j <= p; j += 8) {
-    if (!sees(j)) continue;
-    const int64_t at = paged_row(c, i, h, j);
-    float w = 0.f;
-    for (int r = 0; r < a.rep; ++r) {
-      float q[E];
+  for (int u = threadIdx.x; u < nheads * (HD / 2); u += kPdWarps * 32) {
+    const int r = u / (HD / 2), d = 2 * (u % (HD / 2)), hq = head0 + r;
+    float mm = sm_m[0][r];
 #pragma unroll
-      for (int e = 0; e < E; ++e) q[e] = paged_val(a.q[row * a.q_row + (h * a.rep + r) * a.q_head + lane + 32 * e], c.bf16);
-      const float s = score(q, at);
-      if (sm_m[r] > -INFINITY) w += expf(s - sm_m[r]) * sm_l[r];
+    for (int w = 1; w < kPdWarps; ++w) mm = fmaxf(mm, sm_m[w][r]);
+    if (alone && p.a.sinks) mm = fmaxf(mm, p.a.sinks[hq] * kPdLog2e);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f, vx = 0.f, vy = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPdWarps; ++w) {
+      const float f = exp2f(sm_m[w][r] - ref);
+      const float2 v = *reinterpret_cast<const float2 *>(po + (w * kPdHeads + r) * HD + d);
+      ll += f * sm_l[w][r];
+      vx += f * v.x;
+      vy += f * v.y;
     }
-    if (lane == 0) c.weights[(int64_t(i) * c.kv_heads + h) * c.cap + j] += w;
+    if (alone) {
+      // the heads of one kv head are spread over CTAs: the second kernel adds the weights
+      if (p.accumulate && p.hgroups > 1 && d == 0)
+        *reinterpret_cast<float2 *>(p.part_ml + 2 * (int64_t(i) * p.a.heads + hq) * p.splits) = make_float2(mm, ll);
+      if (p.a.sinks) ll += exp2f(p.a.sinks[hq] * kPdLog2e - ref);
+      const float inv = ll > 0.f ? 1.f / ll : 0.f;
+      *reinterpret_cast<uint32_t *>(p.a.o + i * p.a.o_row + hq * p.a.o_head + d) = pd_pack<BF>(vx * inv, vy * inv);
+      if (d == 0) sm_ml[r] = make_float2(ref, inv);
+    } else {
+      const int64_t at = (int64_t(i) * p.a.heads + hq) * p.splits + split;
+      *reinterpret_cast<float2 *>(p.part_o + at * HD + d) = make_float2(vx, vy);
+      if (d == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(mm, ll);
+    }
   }
+  if (p.accumulate && alone && p.hgroups == 1) {
+    __syncthreads();
+    pd_add_weights(p, sp, i, h, 0, sp.groups, sm_ml);
+  }
+}
+
+// m (log2 units) and 1 / l of a query head over all its splits and its sink; by one warp.
+__device__ __forceinline__ float2 pd_total(const PdArgs &p, int i, int hq, int used, int lane) {
+  const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + (int64_t(i) * p.a.heads + hq) * p.splits;
+  const float sink = p.a.sinks ? p.a.sinks[hq] * kPdLog2e : -INFINITY;
+  float m = sink;
+  for (int s = lane; s < used; s += 32) m = fmaxf(m, ml[s].x);
+  m = warp_max(m);
+  if (m == -INFINITY) return make_float2(0.f, 0.f);
+  float l = 0.f;
+  for (int s = lane; s < used; s += 32) l += exp2f(ml[s].x - m) * ml[s].y;
+  l = warp_sum(l) + exp2f(sink - m);
+  return make_float2(m, 1.f / l);
+}
+
+// Joins the splits of (sequence, kv head): CTAs x < rep the output of query head x, 4 warps taking
+// every fourth split; the others the weights, a share of the groups each.
+template <int HD, bool BF>
+__global__ void __launch_bounds__(kPdWarps * 32) paged_join_kernel(const PdArgs p) {
+  __shared__ float2 sm_ml[128];
+  __shared__ float sm_o[kPdWarps][HD];
+  pdl_trigger();
+  pdl_wait();
+  const int h = blockIdx.y, i = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rep = p.a.rep;
+  const PdSpan sp(paged_len(p.c, i), p.a.window, p.a.first);
+  const int per = sp.per(p.splits), used = max(1, (sp.groups + per - 1) / per);
+  const bool alone = used == 1;
+  if (int(blockIdx.x) < rep) {
+    if (alone) return;  // the first kernel wrote it
+    const int hq = h * rep + blockIdx.x;
+    const float2 tot = pd_total(p, i, hq, used, lane);
+    const int64_t at = (int64_t(i) * p.a.heads + hq) * p.splits;
+    constexpr int E = HD / 32;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll 4
+    for (int s = warp; s < used; s += kPdWarps) {
+      const float f = exp2f(p.part_ml[2 * (at + s)] - tot.x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = fmaf(f, p.part_o[(at + s) * HD + 32 * e + lane], v[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sm_o[warp][32 * e + lane] = v[e] * tot.y;
+    __syncthreads();
+    if (threadIdx.x < HD / 2) {
+      const int d = 2 * threadIdx.x;
+      float x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPdWarps; ++w) {
+        x += sm_o[w][d];
+        y += sm_o[w][d + 1];
+      }
+      *reinterpret_cast<uint32_t *>(p.a.o + i * p.a.o_row + hq * p.a.o_head + d) = pd_pack<BF>(x, y);
+    }
+    return;
+  }
+  if (alone && p.hgroups == 1) return;  // the first kernel added them
+  const int wb = gridDim.x - rep, share = (sp.groups + wb - 1) / wb, g0 = (int(blockIdx.x) - rep) * share;
+  if (g0 >= sp.groups) return;
+  for (int r = warp; r < rep; r += kPdWarps) {
+    const float2 tot = pd_total(p, i, h * rep + r, used, lane);
+    if (lane == 0) sm_ml[r] = tot;
+  }
+  __syncthreads();
+  pd_add_weights(p, sp, i, h, g0, min(sp.groups, g0 + share), sm_ml);
+}
+
+// How a call is cut: by sizes alone, so that its scratch can be asked for beforehand.
+struct PdPlan {
+  int splits, hgroups, wblocks;
+  int64_t score_stride;
+  size_t ml, po, scores;  // bytes
+  bool join;
+};
+
+size_t pd_up(size_t n) { return (n + 255) / 256 * 256; }
+
+PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int max_len, bool accumulate, int sms) {
+  PdPlan p{};
+  p.hgroups = (heads / c.kv_heads + kPdHeads - 1) / kPdHeads;
+  auto groups = [&](int len) -> int64_t {
+    const int64_t all = (int64_t(len) + kPdGroup - 1) / kPdGroup;
+    if (window == 0) return all;
+    return std::min<int64_t>(all, (int64_t(first) + kPdGroup - 1) / kPdGroup + (int64_t(window) + kPdGroup - 1) / kPdGroup + 1);
+  };
+  // The number of splits that makes the longest sequences' CTAs end soonest: waves of CTAs over the SMs
+  // times the rounds (a group a warp) a CTA walks, with a CTA's start and its join counted as
+  // kFixed rounds and the second kernel as as many.
+  constexpr int kFixed = 6;
+  const int64_t units = int64_t(c.seqs) * c.kv_heads * p.hgroups, slots = int64_t(sms) * (c.hd == 128 ? 2 : 3);
+  const int64_t rounds = std::max<int64_t>(1, (groups(max_len) + kPdWarps - 1) / kPdWarps);
+  int64_t best = -1;
+  p.splits = 1;
+  for (int64_t s = 1; s <= std::min<int64_t>(rounds, 256); ++s) {
+    const int64_t per = (rounds + s - 1) / s, real = (rounds + per - 1) / per;
+    if (real != s) continue;
+    const int64_t cost = (units * s + slots - 1) / slots * (per + kFixed) + (s > 1 ? kFixed : 0);
+    if (best < 0 || cost < best) {
+      best = cost;
+      p.splits = int(s);
+    }
+  }
+  p.score_stride = accumulate ? groups(c.cap) * kPdGroup : 0;
+  p.wblocks = accumulate ? int(std::min<int64_t>(64, (groups(max_len) * kPdGroup + 2047) / 2048)) : 0;
+  p.join = p.splits > 1 || (accumulate && p.hgroups > 1);
+  if (p.join) {
+    p.ml = pd_up(size_t(c.seqs) * heads * p.splits * 2 * sizeof(float));
+    p.po = p.splits > 1 ? pd_up(size_t(c.seqs) * heads * p.splits * c.hd * sizeof(float)) : 0;
+  }
+  p.scores = accumulate ? pd_up(size_t(c.seqs) * heads * p.score_stride * sizeof(float)) : 0;
+  return p;
+}
+
+template <int HD, bool BF>
+cudaError_t pd_launch(const PdArgs &p, const PdPlan &plan, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<HD, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       PdRing<HD>::kBytes);
+  if (e != cudaSuccess) return e;
+  launch_pdl(paged_decode_kernel<HD, BF>, dim3(plan.splits, p.c.kv_heads * plan.hgroups, p.c.seqs), dim3(kPdWarps * 32),
+             PdRing<HD>::kBytes, st, p);
+  if (plan.join)
+    launch_pdl(paged_join_kernel<HD, BF>, dim3(p.a.rep + plan.wblocks, p.c.kv_heads, p.c.seqs), dim3(kPdWarps * 32), 0, st,
+               p);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-size_t paged_decode_scratch(const PagedView &, int, int, int, int, bool, int) { return 0; }
-size_t paged_prompt_scratch(const PagedView &, int, int, int, int, int, int, int) { return 0; }
-
-cudaError_t paged_decode(const PagedView &c, const PagedQuery &a, int, bool accumulate, void *, int, cudaStream_t st) {
-  const dim3 grid(1, c.kv_heads, c.seqs);
-  if (c.hd == 128) paged_rows_kernel<128><<<grid, 256, 0, st>>>(c, a, nullptr, c.seqs, 1, accumulate);
-  else paged_rows_kernel<64><<<grid, 256, 0, st>>>(c, a, nullptr, c.seqs, 1, accumulate);
-  return cudaGetLastError();
+size_t paged_decode_scratch(const PagedView &c, int heads, int window, int first, int max_len, bool accumulate, int sms) {
+  const PdPlan p = pd_plan(c, heads, window, first, max_len, accumulate, sms);
+  return p.ml + p.po + p.scores;
 }
 
-cudaError_t paged_prompt(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows, int max_rows, int,
-                         void *, int, cudaStream_t st) {
-  const dim3 grid(max_rows, c.kv_heads, c.seqs);
-  if (c.hd == 128) paged_rows_kernel<128><<<grid, 256, 0, st>>>(c, a, starts, rows, max_rows, false);
-  else paged_rows_kernel<64><<<grid, 256, 0, st>>>(c, a, starts, rows, max_rows, false);
-  return cudaGetLastError();
+cudaError_t paged_decode(const PagedView &c, const PagedQuery &a, int max_len, bool accumulate, void *scratch, int sms,
+                         cudaStream_t st) {
+  const PdPlan plan = pd_plan(c, a.heads, a.window, a.first, max_len, accumulate, sms);
+  uint8_t *base = static_cast<uint8_t *>(scratch);
+  const PdArgs p{c, a, plan.splits, plan.hgroups, accumulate, plan.score_stride, reinterpret_cast<float *>(base),
+                 reinterpret_cast<float *>(base + plan.ml), reinterpret_cast<float *>(base + plan.ml + plan.po)};
+  if (c.hd == 128) return c.bf16 ? pd_launch<128, true>(p, plan, st) : pd_launch<128, false>(p, plan, st);
+  return c.bf16 ? pd_launch<64, true>(p, plan, st) : pd_launch<64, false>(p, plan, st);
 }
 
 }  // namespace hc
