@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "paged.h"
 
 namespace hc {
 
@@ -205,6 +206,8 @@ HC_API char *hc_device_check(hc_device *d) {
   HC_TRY_CUDA(cudaDeviceSynchronize());
   const int code = hc::tc_status_take();
   if (code) return hc::make_error("a tensor-core GEMV wait ran out (code " + std::to_string(code) + ")");
+  const int prompt = hc::paged_status_take();
+  if (prompt) return hc::make_error("a wait of the paged prompt attention ran out (code " + std::to_string(prompt) + ")");
   return nullptr;
 }
 

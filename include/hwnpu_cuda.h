@@ -79,9 +79,10 @@ HC_API void hc_device_free(hc_device *d);
  * bytes; *need is its length with the NUL. */
 HC_API char *hc_device_info(hc_device *d, int key, char *buf, size_t n, size_t *need);
 /* Health of the library's kernels on the device: an error string when a bounded wait inside one of
- * them (the tensor-core GEMV's pipeline waits, about a second each) ran out since the last call --
- * the results of that launch are not to be trusted -- else NULL; clears the record. Waits for the
- * device's queued work first. (The reference's xs_run_wait reports a failed run the same way.) */
+ * them (the pipeline waits of the tensor-core GEMV and of the paged prompt attention, about a second
+ * each) ran out since the last call -- the results of that launch are not to be trusted -- else NULL;
+ * clears the record. Waits for the device's queued work first. (The reference's xs_run_wait reports a
+ * failed run the same way.) */
 HC_API char *hc_device_check(hc_device *d);
 
 /* ---------------------------------------------------------------------------------------- */
