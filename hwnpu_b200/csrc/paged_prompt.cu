@@ -12,7 +12,7 @@
 // sequence: while the softmax of one runs, the tensor cores work for the other.
 //
 // Slots come in groups of 16 aligned ones, each inside one page, so a tile of 128 slots is eight TMA
-// boxes a 64-column half, from wherever the pages are: first the groups of the first tokens that stay
+// boxes (a 64-column half for K), from wherever the pages are: first the groups of the first tokens that stay
 // visible, then those from the lowest slot any row of the CTA sees to its last token. No tile is
 // spent on the slots between. Rows of an edge group that no row of the CTA sees are zeroed in shared
 // memory (values only: a hidden score is replaced, but 0 times a hidden NaN would not be 0).
@@ -20,7 +20,7 @@
 //   warps 0-3, 4-7  softmax of tile A, B: a thread owns a row. It reads the row's 128 scores from tensor
 //                   memory, keeps the running maximum and sum in float32, writes P back as 16-bit
 //                   values over the scores, and at the end O / l to memory
-//   warp 8          copies the groups (cp.async.bulk.tensor, an mbarrier a ring stage)
+//   warps 8, 10     copy the groups of K, of V (cp.async.bulk.tensor, an mbarrier a ring stage)
 //   warp 9          issues the MMAs: S = Q K^T (both operands in shared memory, 128-byte swizzle),
 //                   O += P V (P in tensor memory, V in shared memory, MN-major)
 //
@@ -65,6 +65,9 @@ template <int HD>
 struct PpSmem {
   static constexpr int kHalves = HD / 64;
   static constexpr int kTile = kHalves * kPpHalf;  // Q of a tile, or K or V of 128 slots
+  // V of a group, [half][16 rows][128 bytes]: a group is one K-step of P V, so its halves may lie together
+  static constexpr int kVHalf = kPpGroup * 128;
+  static constexpr int kVGroup = kHalves * kVHalf;
   static constexpr int kStages = HD == 128 ? 5 : 10;
   static constexpr int kBytes = (2 + kStages) * kTile + 1024;
 };
@@ -89,7 +92,7 @@ __device__ __forceinline__ void pp_wait(uint64_t *b, unsigned parity, volatile i
 }
 
 // Shared-memory descriptors with the 128-byte swizzle (8 rows x 128 bytes an atom): K-major (rows are M or
-// N, 8-row groups 1,024 bytes apart), and MN-major (rows are K; the next 64 columns kPpHalf further).
+// N, 8-row groups 1,024 bytes apart), and MN-major (rows are K; the next 64 columns lbo further).
 __device__ __forceinline__ uint64_t pp_desc(uint32_t saddr, uint32_t lbo) {
   return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(lbo >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
          (uint64_t(1) << 46) | (uint64_t(2) << 61);
@@ -108,12 +111,21 @@ __device__ __forceinline__ void pp_mma_ta(uint32_t d, uint32_t a, uint64_t bdesc
       "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void pp_tma(uint32_t dst, const CUtensorMap *map, int col, int row, int head, int page,
-                                       uint64_t *bar) {
+// A box of 16 rows: of K 64 columns, of V all of them as 64-column halves one behind the other.
+__device__ __forceinline__ void pp_tma_k(uint32_t dst, const CUtensorMap *map, int col, int row, int head, int page,
+                                         uint64_t *bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
       "[%6];" ::"r"(dst),
       "l"(map), "r"(col), "r"(row), "r"(head), "r"(page), "r"(tc_saddr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void pp_tma_v(uint32_t dst, const CUtensorMap *map, int row, int head, int page,
+                                         uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(tc_saddr(bar))
       : "memory");
 }
 // 128 columns of this warp's 32 lanes of tensor memory, waited for.
@@ -304,52 +316,58 @@ __global__ void __launch_bounds__(kPpThreads, 1)
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpRestRegs));
-    if (warp == 8) {
-      // K and V of each tile, a ring stage each; lane l copies half l % halves of group l / halves
+    if (warp == 8 || warp == 10) {
+      // the K (warp 8) or V (warp 10) of each tile, in every other ring stage: for K lane l copies half
+      // l % halves of group l / halves, for V lane l both halves of group l
+      const bool val = warp == 10;
       const int32_t *table = p.c.table + i * p.c.table_stride;
-      const int mask = (1 << p.c.shift) - 1, gi = lane / Sm::kHalves, hf = lane % Sm::kHalves;
+      const int mask = (1 << p.c.shift) - 1, gi = val ? lane : lane / Sm::kHalves, hf = val ? 0 : lane % Sm::kHalves;
       auto page_of = [&](int j) {
         const int g = j * kPpGroups + gi;
         return j < j1 && gi < kPpGroups && g < sp.groups ? table[sp.slot(g) >> p.c.shift] : -1;
       };
-      int page = page_of(j0), fills = 0;
-      for (int j = j0; j < j1; ++j) {
+      int page = page_of(j0), fill = val ? 1 : 0;
+      for (int j = j0; j < j1; ++j, fill += 2) {
         const int next = page_of(j + 1);
         const int ng = min(kPpGroups, sp.groups - j * kPpGroups);
         const int slot = gi < ng ? sp.slot(j * kPpGroups + gi) : 0;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++fills) {
-          const int s = fills % ST;
-          if (fills >= ST) pp_wait(&empty[s], (fills / ST - 1) & 1, dead, 11);
-          if (*dead) break;
-          if (lane == 0) tc_expect_tx(&full[s], unsigned(ng * kPpGroup * HD * 2));
-          __syncwarp();
-          if (gi < ng)
-            pp_tma(tc_saddr(ring + s * Sm::kTile + hf * kPpHalf + gi * (kPpGroup * 128)), kv ? &vmap : &kmap, hf * 64,
-                   slot & mask, h, page, &full[s]);
-        }
+        const int s = fill % ST;
+        if (fill >= ST) pp_wait(&empty[s], (fill / ST - 1) & 1, dead, 11);
         if (*dead) break;
+        if (lane == 0) tc_expect_tx(&full[s], unsigned(ng * kPpGroup * HD * 2));
+        __syncwarp();
+        const uint32_t dst = tc_saddr(ring + s * Sm::kTile);
+        if (gi < ng) {
+          if (val) pp_tma_v(dst + gi * Sm::kVGroup, &vmap, slot & mask, h, page, &full[s]);
+          else pp_tma_k(dst + hf * kPpHalf + gi * (kPpGroup * 128), &kmap, hf * 64, slot & mask, h, page, &full[s]);
+        }
         page = next;
       }
       // after a wait that ran out: no copy may be in flight when the CTA ends
       if (*dead)
-        for (int f = max(0, fills - ST); f < fills; ++f) tc_wait(&full[f % ST], (f / ST) & 1, &pp_status_word, 12);
+        for (int f = max(val ? 1 : 0, fill - 2 * ST); f < fill; f += 2)
+          tc_wait(&full[f % ST], (f / ST) & 1, &pp_status_word, 12);
     } else if (warp == 9) {
-      const uint32_t q0 = tc_saddr(qsm), r0 = tc_saddr(ring);
+      // descriptors of the first K-step; the others differ in the address (units of 16 bytes)
+      const uint64_t qd[2] = {pp_desc(tc_saddr(qsm), 16), pp_desc(tc_saddr(qsm) + Sm::kTile, 16)};
+      const uint64_t kd = pp_desc(tc_saddr(ring), 16), vd = pp_desc(tc_saddr(ring), Sm::kVHalf);
+      const uint32_t idv = pp_idesc(BF, HD, true);
       auto scores = [&](int x, int s, int ng) {  // S_x = Q_x K^T of the stage's ng groups
         const uint32_t id = pp_idesc(BF, ng * kPpGroup, false);
+        const uint64_t kb = kd + s * (Sm::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (k >> 2) * kPpHalf + (k & 3) * 32;
-          tc_mma(tmem + x * 128, pp_desc(q0 + x * Sm::kTile + off, 16), pp_desc(r0 + s * Sm::kTile + off, 16), id, k > 0);
+          const uint32_t off = ((k >> 2) * kPpHalf + (k & 3) * 32) >> 4;
+          tc_mma(tmem + x * 128, qd[x] + off, kb + off, id, k > 0);
         }
         tc_commit(&sfull[x]);
       };
       auto values = [&](int x, int s, int ng, bool add) {  // O_x += P_x V
-        const uint32_t id = pp_idesc(BF, HD, true);
-        for (int k = 0; k < ng; ++k)
-          pp_mma_ta(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, pp_desc(r0 + s * Sm::kTile + k * (kPpGroup * 128), kPpHalf),
-                    id, add || k > 0);
+        const uint64_t vb = vd + s * (Sm::kTile >> 4);
+#pragma unroll
+        for (int k = 0; k < kPpGroups; ++k)
+          if (k < ng)
+            pp_mma_ta(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, vb + k * (Sm::kVGroup >> 4), idv, add || k > 0);
         tc_commit(&ofull[x]);
       };
       auto groups_of = [&](int j) { return min(kPpGroups, sp.groups - j * kPpGroups); };
@@ -369,19 +387,20 @@ __global__ void __launch_bounds__(kPpThreads, 1)
         const int j = j0 + u, ng = groups_of(j), fv = 2 * u + 1, fk = 2 * u + 2;
         pp_wait(&full[fv % ST], (fv / ST) & 1, dead, 15);
         // values of slots that no row of this CTA sees
-        bool zeroed = false;
-        for (int g = 0; g < ng; ++g) {
-          const int s0 = sp.slot(j * kPpGroups + g);
-          if (s0 + kPpGroup - 1 <= pmax && (s0 >= sp.lo || s0 + kPpGroup <= sp.first)) continue;
-          zeroed = true;
-          for (int e = lane; e < kPpGroup * Sm::kHalves * 8; e += 32) {
-            const int r = e / (Sm::kHalves * 8), ch = e % (Sm::kHalves * 8), s = s0 + r;
-            if (s > pmax || (s < sp.lo && s >= sp.first))
-              *reinterpret_cast<uint4 *>(ring + (fv % ST) * Sm::kTile + (ch >> 3) * kPpHalf + (g * kPpGroup + r) * 128 +
-                                         (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+        const int jb = sp.slot(j * kPpGroups), je = sp.slot(j * kPpGroups + ng - 1) + kPpGroup;
+        if (je - 1 > pmax || (jb < sp.lo && je > sp.first)) {
+          for (int g = 0; g < ng; ++g) {
+            const int s0 = sp.slot(j * kPpGroups + g);
+            if (s0 + kPpGroup - 1 <= pmax && (s0 >= sp.lo || s0 + kPpGroup <= sp.first)) continue;
+            for (int e = lane; e < kPpGroup * Sm::kHalves * 8; e += 32) {
+              const int r = e / (Sm::kHalves * 8), ch = e % (Sm::kHalves * 8), s = s0 + r;
+              if (s > pmax || (s < sp.lo && s >= sp.first))
+                *reinterpret_cast<uint4 *>(ring + (fv % ST) * Sm::kTile + g * Sm::kVGroup + (ch >> 3) * Sm::kVHalf +
+                                           r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
           }
+          tc_fence_proxy();
         }
-        if (zeroed) tc_fence_proxy();
         if (u + 1 < n) pp_wait(&full[fk % ST], (fk / ST) & 1, dead, 16);
         __syncwarp();
         for (int x = 0; x < (two ? 2 : 1); ++x) {
@@ -593,18 +612,22 @@ EncodeFn pp_encoder() {
   return reinterpret_cast<EncodeFn>(f);
 }
 
-// The pool as (column, row of a page, head, page), a box of 16 rows x 64 columns, 128-byte swizzle; what
-// lies outside reads as zeros.
-bool pp_map(EncodeFn enc, const PagedView &c, const uint16_t *base, CUtensorMap *map) {
-  const cuuint64_t dims[4] = {cuuint64_t(c.hd), cuuint64_t(1) << c.shift, cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
+// The pool as (column, row of a page, head, page), a box of 16 rows x 64 columns (K), or as (column of a
+// half, row, half, head, page), a box of 16 rows x all columns, half by half (V); 128-byte swizzle, and
+// what lies outside reads as zeros.
+bool pp_map(EncodeFn enc, const PagedView &c, bool halves, CUtensorMap *map) {
   const cuuint64_t row = cuuint64_t(c.row_stride) * 2;
   // a dimension of one has no stride of its own
-  const cuuint64_t strides[3] = {row, c.kv_heads > 1 ? cuuint64_t(c.head_stride) * 2 : row,
-                                 c.pages > 1 ? cuuint64_t(c.page_stride) * 2 : row};
-  const cuuint32_t box[4] = {64, kPpGroup, 1, 1}, step[4] = {1, 1, 1, 1};
-  return enc(map, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-             const_cast<uint16_t *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const cuuint64_t head = c.kv_heads > 1 ? cuuint64_t(c.head_stride) * 2 : row;
+  const cuuint64_t page = c.pages > 1 ? cuuint64_t(c.page_stride) * 2 : row;
+  const cuuint64_t rows = cuuint64_t(1) << c.shift, heads = cuuint64_t(c.kv_heads), pages = cuuint64_t(c.pages);
+  const cuuint64_t kdims[4] = {cuuint64_t(c.hd), rows, heads, pages}, kstr[3] = {row, head, page};
+  const cuuint64_t vdims[5] = {64, rows, cuuint64_t(c.hd / 64), heads, pages}, vstr[4] = {row, 128, head, page};
+  const cuuint32_t kbox[4] = {64, kPpGroup, 1, 1}, vbox[5] = {64, kPpGroup, cuuint32_t(c.hd / 64), 1, 1};
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  return enc(map, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, halves ? 5 : 4,
+             halves ? c.v : c.k, halves ? vdims : kdims, halves ? vstr : kstr, halves ? vbox : kbox, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -678,7 +701,7 @@ cudaError_t paged_prompt(const PagedView &c, const PagedQuery &a, const int32_t 
   EncodeFn enc = pp_encoder();
   if (!enc) return cudaErrorNotSupported;
   CUtensorMap km, vm;
-  if (!pp_map(enc, c, c.k, &km) || !pp_map(enc, c, c.v, &vm)) return cudaErrorInvalidValue;
+  if (!pp_map(enc, c, false, &km) || !pp_map(enc, c, true, &vm)) return cudaErrorInvalidValue;
   uint8_t *base = static_cast<uint8_t *>(scratch);
   const PpArgs p{c, a, starts, rows, max_rows, plan.tokens, plan.blocks, plan.splits, reinterpret_cast<float *>(base),
                  reinterpret_cast<float *>(base + plan.ml)};
