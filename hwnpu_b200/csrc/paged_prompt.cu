@@ -8,29 +8,36 @@
 // values are read from HBM once and from the L2 cache by every CTA.
 //
 // Rows. The query heads of a kv head share its keys, so a tile's 128 rows are 128 / rep tokens x rep heads
-// (row = token * rep + head). A CTA owns two such tiles (A and B), consecutive tokens of one
+// (row = token * rep + head). A block of rows is two such tiles (A and B), consecutive tokens of one
 // sequence: while the softmax of one runs, the tensor cores work for the other.
 //
-// Slots come in groups of 16 aligned ones, each inside one page, so a tile of 128 slots is eight TMA
-// boxes (a 64-column half for K), from wherever the pages are: first the groups of the first tokens that stay
-// visible, then those from the lowest slot any row of the CTA sees to its last token. No tile is
-// spent on the slots between. Rows of an edge group that no row of the CTA sees are zeroed in shared
+// Slots come in groups of 16 aligned ones, each inside one page, so a tile of 128 slots is one to
+// eight TMA boxes (a 64-column half for K), from wherever the pages are: first the groups of the first tokens that stay
+// visible, then those from the lowest slot any row of the block sees to its last token. No tile is
+// spent on the slots between. Rows of an edge group that no row of the block sees are zeroed in shared
 // memory (values only: a hidden score is replaced, but 0 times a hidden NaN would not be 0).
+//
+// Work. One CTA an SM. All blocks of all heads and sequences, as many tiles long as they see (and one
+// more for a block's start and end), lie one behind the other, and every CTA takes an equal part of that
+// line, read from the lengths on the device: ragged sequences, causal triangles and few rows over a
+// long cache come out even. A block that a cut falls into is finished by a second kernel, which
+// joins the parts' (m, l, O) in order.
 //
 //   warps 0-3, 4-7  softmax of tile A, B: a thread owns a row. It reads the row's 128 scores from tensor
 //                   memory, keeps the running maximum and sum in float32, writes P back as 16-bit
-//                   values over the scores, and at the end O / l to memory
-//   warps 8, 10     copy the groups of K, of V (cp.async.bulk.tensor, an mbarrier a ring stage)
-//   warp 9          issues the MMAs: S = Q K^T (both operands in shared memory, 128-byte swizzle),
-//                   O += P V (P in tensor memory, V in shared memory, MN-major)
+//                   values over the scores (a half of the slots at a time, so that P V of the first
+//                   runs beside the exponentials of the second), and at the end O / l to memory
+//   warp 8          copies the groups of K and V (cp.async.bulk.tensor, an mbarrier a ring stage)
+//   warps 9, 10     issue the MMAs of tile A, B: S = Q K^T (both operands in shared memory, 128-byte
+//                   swizzle), O += P V (P in tensor memory, V in shared memory, MN-major)
+//   warp 11         walks the CTA's part of the line, a block ahead of the others, and copies Q
+// The next block's K, V, Q and first scores are under way while a block's last tile and output are.
 //
 // Arithmetic. S and O are float32. P = exp2(S scale log2(e) - m) is rounded to the cache's type (the MMA
 // wants it of V's type); l sums it unrounded in float32. m is moved only when a score passes it by more
 // than 2^8, which rescales O in tensor memory; P is at most 256 then, and fp16's P is held 2^7 higher
-// so that its smallest weights stand for 2^-32.
-//
-// Few rows over a long cache: the tiles of a CTA's rows are split over further CTAs, whose unfinished
-// (m, l, O) a second kernel joins, in order.
+// so that its smallest weights stand for 2^-32. (A polynomial for some of the exponentials, on the FMA
+// pipes, was slower: 617 us against 583 for the 16,384-token prompt with a quarter of them.)
 //
 // Every mbarrier wait is bounded (about a second of SM clocks): one that runs out records a code that
 // hc_device_check reports and lets every other wait of the CTA return; the CTA still waits, bounded,
@@ -52,24 +59,24 @@ constexpr int kPpRows = 128;               // rows of a tile (the MMA's M)
 constexpr int kPpSlots = 128;              // slots of a tile
 constexpr int kPpGroup = 16;               // slots of a group (one TMA box, one K-step of P V)
 constexpr int kPpGroups = kPpSlots / kPpGroup;
-constexpr int kPpThreads = 384;            // three warpgroups: softmax of A, of B, and the rest
-// Registers a thread: launched with 168 (65,536 / 384), then 224 for the softmax and 56 for the rest, which
-// adds up to the same (2 x 224 + 56 = 3 x 168).
-constexpr int kPpSoftRegs = 224, kPpRestRegs = 56;
+constexpr int kPpSoft = 256;               // threads of the softmax, one a row
+constexpr int kPpThreads = kPpSoft + 128;
+// Registers a thread: launched with 168 (65,536 / 384), then 208 for the softmax and 88 for the rest, which
+// adds up to the same (2 x 208 + 88 = 3 x 168).
+constexpr int kPpSoftRegs = 208, kPpRestRegs = 88;
 constexpr int kPpHalf = kPpRows * 128;     // bytes of 128 rows x 64 columns
 constexpr float kPpLazy = 8.f;
 constexpr float kPpLog2e = 1.4426950408889634f;
 constexpr uint32_t kPpTmem = 512;          // columns: S_A, S_B (128 each), O_A, O_B
+constexpr int kPpSegs = 4;                 // blocks the walking warp may be ahead
+constexpr int kPpMinPart = 4;              // least tiles of a CTA's part of the line
 
 template <int HD>
 struct PpSmem {
   static constexpr int kHalves = HD / 64;
   static constexpr int kTile = kHalves * kPpHalf;  // Q of a tile, or K or V of 128 slots
-  // V of a group, [half][16 rows][128 bytes]: a group is one K-step of P V, so its halves may lie together
-  static constexpr int kVHalf = kPpGroup * 128;
-  static constexpr int kVGroup = kHalves * kVHalf;
   static constexpr int kStages = HD == 128 ? 5 : 10;
-  static constexpr int kBytes = (2 + kStages) * kTile + 1024;
+  static constexpr int kBytes = (2 + kStages) * kTile;  // 224 KB with head_dim 128: 3 KB are left
 };
 
 __device__ int pp_status_word;  // the first wait that ran out in any launch (0: none)
@@ -120,6 +127,7 @@ __device__ __forceinline__ void pp_tma_k(uint32_t dst, const CUtensorMap *map, i
       "l"(map), "r"(col), "r"(row), "r"(head), "r"(page), "r"(tc_saddr(bar))
       : "memory");
 }
+// (pp_tma_k also copies Q: a box of tokens x rep heads.)
 __device__ __forceinline__ void pp_tma_v(uint32_t dst, const CUtensorMap *map, int row, int head, int page,
                                          uint64_t *bar) {
   asm volatile(
@@ -128,7 +136,7 @@ __device__ __forceinline__ void pp_tma_v(uint32_t dst, const CUtensorMap *map, i
       "l"(map), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(tc_saddr(bar))
       : "memory");
 }
-// 128 columns of this warp's 32 lanes of tensor memory, waited for.
+// 128 columns of this warp's 32 lanes of tensor memory (a lane a row), waited for.
 __device__ __forceinline__ void pp_ld128(uint32_t taddr, uint32_t (&r)[128]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
@@ -142,38 +150,35 @@ __device__ __forceinline__ void pp_ld128(uint32_t taddr, uint32_t (&r)[128]) {
       "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
       "}, [%128];\n tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-      "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-      "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-      "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
-      "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]),
-      "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]),
-      "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]),
-      "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-      "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
-      "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]),
-      "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]),
-      "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]),
-      "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]),
-      "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]),
-      "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]),
+        "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]),
+        "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
+        "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]),
+        "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]),
+        "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]),
+        "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]),
+        "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]),
+        "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
       : "r"(taddr)
       : "memory");
 }
-// 32 columns, waited for.
-__device__ __forceinline__ void pp_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
-      "}, [%32];\n tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-      "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-      "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-      "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
+      "};"
+      :
+      : "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t *r) {
+__device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -181,12 +186,51 @@ __device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t *r) {
       "};"
       :
       : "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+// 32 columns of 16 lanes as an MMA's fragment, waited for: r[4 i + e] is column 8 i + 2 (lane % 4) + e % 2 of
+// row lane / 4 + 8 (e / 2).
+__device__ __forceinline__ void pp_ldo(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
+      "}, [%16];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void pp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- two floats a register pair
+__device__ __forceinline__ uint64_t pp_two(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 pp_split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t pp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t pp_add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float pp_max3(float a, float b, float c) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
 
 __device__ __forceinline__ float pp_exp2(float x) {
   float y;
@@ -204,267 +248,534 @@ __device__ __forceinline__ uint32_t pp_pack(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&x);
 }
 
-// The rows of a CTA and the slots they see: tokens [t0, t1) of sequence i, the token t at slot
-// p0 + t, as groups of 16 slots: ga of them from slot 0 on, then those from slot 16 b0 on.
+// Byte offset of V's row r (a multiple of 8) and 64-column half in a stage: boxes one behind the other, in a box
+// the halves, in a half its rows of 128 bytes.
+template <int HD>
+__device__ __forceinline__ int pp_voff(int r, int half, int box) {
+  return (r & -box) * (HD * 2) + half * box * 128 + (r & (box - 1)) * 128;
+}
+
+// A block of rows and the slots they see: tokens [t0, t1) of a sequence, the token t at slot p0 + t, as
+// groups of 16 slots: ga of them from slot 0 on, then those from slot 16 b0 on.
 struct PpSpan {
   int row0, t0, t1, p0;          // row0: the q row of token 0
   int lo, first, ga, b0, groups;
-  // false: nothing to do
+  // false: no such block
   __device__ __forceinline__ bool set(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows,
-                                      int max_rows, int i, int tokens, int block) {
+                                      int max_rows, int i, int tokens, int block, int box) {
     row0 = starts[i];
     const int cnt = starts[i + 1] - row0;
     if (row0 < 0 || row0 > rows || cnt <= 0) return false;
+    const int last = min(min(cnt, max_rows), rows - row0);
+    if (int64_t(block) * tokens >= last) return false;
     t0 = block * tokens;
-    t1 = min(min(t0 + tokens, min(cnt, max_rows)), rows - row0);
-    if (t0 >= t1) return false;
+    t1 = last - t0 > tokens ? t0 + tokens : last;
     p0 = paged_len(c, i) - cnt;
     const int pmin = p0 + t0, pmax = p0 + t1 - 1;
     lo = a.window > 0 && pmin >= a.window ? pmin - a.window + 1 : 0;
     first = min(a.first, lo);
-    ga = (first + kPpGroup - 1) / kPpGroup;
-    b0 = max(lo / kPpGroup, ga);
+    // both runs of groups begin at a box's first row (box is a power of two), so no box is cut by a tile's end
+    ga = ((first + box - 1) & -box) / kPpGroup;
+    b0 = max((lo & -box) / kPpGroup, ga);
     groups = pmax < 0 ? 0 : ga + pmax / kPpGroup + 1 - b0;
     return true;
   }
   __device__ __forceinline__ int slot(int g) const { return (g < ga ? g : g - ga + b0) * kPpGroup; }
   __device__ __forceinline__ int tiles() const { return (groups + kPpGroups - 1) / kPpGroups; }
-  // tiles of one split when the work is cut in up to `splits`
-  __device__ __forceinline__ int per(int splits) const { return max(1, (tiles() + splits - 1) / splits); }
+};
+
+// What a CTA does of one block: tiles [j0, j1) of sequence i, kv head h (-1: the CTA's part is done).
+struct PpSeg : PpSpan {
+  int i, h, j0, j1;
+  int part;  // where unfinished rows go; -1: these are all the block's tiles, the output is written
+};
+
+// The block whose first tiles a CTA has and whose last ones it has not: its parts are those of this
+// CTA and the `parts` - 1 after it (0: there is none).
+struct PpHead {
+  int parts, row0, t0, t1, h, pad[3];
 };
 
 struct PpArgs {
   PagedView c;
   PagedQuery a;
   const int32_t *starts;
-  int rows, max_rows, tokens, blocks, splits;  // tokens: of a tile (128 / rep); blocks: of two tiles
-  float *part_ml;                              // [rows][heads][splits][2]: reference (log2 units) and l
-  float *part_o;                               // [rows][heads][splits][hd], not divided by l
+  int rows, max_rows, tokens, blocks, slot_rows;  // tokens: of a tile (128 / rep); blocks: of two tiles, a sequence
+  int box;                                        // rows of a TMA box: 16 to 128, at most a page
+  PpHead *heads;                                  // [CTAs]
+  float2 *part_ml;                                // [2 CTAs][slot_rows]: reference (log2 units) and l
+  float *part_o;                                  // [2 CTAs][slot_rows][hd], not divided by l
 };
 
-// Copies 128 rows of Q (token-major, heads within) into the swizzled operand; rows past the last token
-// are zeros. flip: the sign of a negative scale, which the softmax takes as positive.
-template <int HD>
-__device__ __forceinline__ void pp_load_q(const PpArgs &p, const PpSpan &sp, int h, int t0, uint8_t *dst, int tid) {
-  constexpr int CH = HD / 8;
-  const uint32_t flip = p.a.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll 4
-  for (int u = tid; u < kPpRows * CH; u += kPpRows) {
-    const int r = u / CH, ch = u % CH, t = r / p.a.rep, hq = h * p.a.rep + r % p.a.rep;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (t < p.tokens && t0 + t < sp.t1) {
-      v = *reinterpret_cast<const uint4 *>(p.a.q + int64_t(sp.row0 + t0 + t) * p.a.q_row + hq * p.a.q_head + 8 * ch);
-      v.x ^= flip;
-      v.y ^= flip;
-      v.z ^= flip;
-      v.w ^= flip;
+// The line of blocks of one kv head, from sequence 0's first to the last's last; place u is block
+// u % blocks of sequence u / blocks, and a place without rows has no length.
+__device__ __forceinline__ bool pp_place(const PpArgs &p, int64_t u, PpSpan *sp) {
+  return sp->set(p.c, p.a, p.starts, p.rows, p.max_rows, int(u / p.blocks), 2 * p.tokens, int(u % p.blocks), p.box);
+}
+
+struct PpShare {
+  long long head_len, part, begin, end;  // of one kv head's line, of a CTA's part; this CTA's part
+  long long place;                       // where begin falls into the line of its head
+  int off;                               // and how many tiles into that block
+};
+
+// Measures the line and finds this CTA's part of it (the same on every CTA); all threads.
+__device__ __forceinline__ void pp_share(const PpArgs &p, PpShare *sh, long long *sums) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t n = int64_t(p.c.seqs) * p.blocks, each = (n + kPpThreads - 1) / kPpThreads;
+  const int64_t u0 = min(n, tid * each), u1 = min(n, u0 + each);
+  long long own = 0;
+  PpSpan sp;
+  for (int64_t u = u0; u < u1;) {
+    if (pp_place(p, u, &sp)) {
+      own += sp.tiles() + 1;
+      ++u;
+    } else {
+      u = (u / p.blocks + 1) * p.blocks;  // no further block of this sequence either
     }
-    *reinterpret_cast<uint4 *>(dst + (ch >> 3) * kPpHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+  }
+  long long upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < kPpThreads / 32; ++w) {
+    before += w < warp ? sums[w] : 0;
+    total += sums[w];
+  }
+  const long long line = total * p.c.kv_heads;
+  const long long part = max((long long)kPpMinPart, (line + gridDim.x - 1) / gridDim.x);
+  const long long begin = min(line, blockIdx.x * part), end = min(line, begin + part);
+  if (tid == 0) {
+    sh->head_len = total;
+    sh->part = part;
+    sh->begin = begin;
+    sh->end = end;
+  }
+  if (begin >= end) return;
+  long long at = before + upto - own;  // where this thread's places begin
+  const long long want = begin % total;
+  if (want < at || want >= at + own) return;
+  for (int64_t u = u0; u < u1;) {
+    if (pp_place(p, u, &sp)) {
+      const int len = sp.tiles() + 1;
+      if (want < at + len) {
+        sh->place = u;
+        sh->off = int(want - at);
+        return;
+      }
+      at += len;
+      ++u;
+    } else {
+      u = (u / p.blocks + 1) * p.blocks;
+    }
   }
 }
 
 template <int HD, bool BF>
 __global__ void __launch_bounds__(kPpThreads, 1)
-    paged_prompt_kernel(const PpArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    paged_prompt_kernel(const PpArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                        const __grid_constant__ CUtensorMap qmap) {
   using Sm = PpSmem<HD>;
   constexpr int ST = Sm::kStages;
-  extern __shared__ uint8_t pp_raw[];
-  __shared__ uint64_t full[ST], empty[ST], qfull, sfull[2], pfull[2], ofull[2], done;
+  constexpr int kCopy = kPpSoft / 32, kMma = kCopy + 1, kWalk = kCopy + 3;  // warps
+  extern __shared__ __align__(1024) uint8_t pp_sm[];  // the swizzle counts from 1,024-byte lines
+  __shared__ uint64_t full[ST], empty[ST], vland, qfull, qempty, segfull[kPpSegs], segempty[kPpSegs];
+  __shared__ uint64_t sfull[2], pfull[2][2], ofull[2], ofree[2], exp_turn[2][4], done[2];
+  __shared__ PpSeg segs[kPpSegs];
+  __shared__ PpShare share;
+  __shared__ long long sums[kPpThreads / 32];
   __shared__ uint32_t tmem_base;
   __shared__ int dead_flag;
   pdl_trigger();
-  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y, i = blockIdx.z;
-  // the last tokens see the most: their CTAs start first
-  const int block = p.blocks - 1 - int(blockIdx.x) / p.splits, split = int(blockIdx.x) % p.splits;
-  PpSpan sp;
-  if (!sp.set(p.c, p.a, p.starts, p.rows, p.max_rows, i, 2 * p.tokens, block)) return;
-  const int per = sp.per(p.splits), tiles = sp.tiles();
-  const int j0 = split * per, j1 = min(tiles, j0 + per);
-  if (j0 >= j1 && split > 0) return;
-  const bool alone = tiles <= per;
-  const bool two = sp.t1 - sp.t0 > p.tokens;  // tile B has rows
-  uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pp_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *qsm = sm, *ring = sm + 2 * Sm::kTile;
+  uint8_t *qsm = pp_sm, *ring = pp_sm + 2 * Sm::kTile;
   volatile int *dead = &dead_flag;
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       tc_bar_init(&full[s], 1);
-      tc_bar_init(&empty[s], 1);
+      tc_bar_init(&empty[s], 2);  // both tiles' MMAs
     }
-    tc_bar_init(&qfull, two ? 8 : 4);
+    tc_bar_init(&vland, 1);
+    tc_bar_init(&qfull, 1);
+    tc_bar_init(&qempty, 2);
+    for (int s = 0; s < kPpSegs; ++s) {
+      tc_bar_init(&segfull[s], 1);
+      tc_bar_init(&segempty[s], kPpThreads / 32 - 1);  // every warp but the one that fills them
+    }
     for (int x = 0; x < 2; ++x) {
       tc_bar_init(&sfull[x], 1);
-      tc_bar_init(&pfull[x], 4);
+      tc_bar_init(&pfull[x][0], 4);  // a half of the slots each
+      tc_bar_init(&pfull[x][1], 4);
+      for (int w = 0; w < 4; ++w) tc_bar_init(&exp_turn[x][w], 1);
       tc_bar_init(&ofull[x], 1);
+      tc_bar_init(&ofree[x], 4);
     }
-    tc_bar_init(&done, 1);
+    tc_bar_init(&done[0], 1);
+    tc_bar_init(&done[1], 1);
     dead_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_saddr(&tmem_base)),
                  "r"(kPpTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  pdl_wait();
+  pp_share(p, &share, sums);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
+  // block k of the CTA's part, once warp 11 has it; seg_done gives its place back
+  auto seg_get = [&](int k) -> const PpSeg & {
+    pp_wait(&segfull[k % kPpSegs], (k / kPpSegs) & 1, dead, 11);
+    return segs[k % kPpSegs];
+  };
+  auto seg_done = [&](int k) {
+    __syncwarp();
+    if (lane == 0) tc_arrive(&segempty[k % kPpSegs]);
+  };
 
-  if (warp >= 8) {
+  if (warp >= kPpSoft / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpRestRegs));
-    if (warp == 8 || warp == 10) {
-      // the K (warp 8) or V (warp 10) of each tile, in every other ring stage: for K lane l copies half
-      // l % halves of group l / halves, for V lane l both halves of group l
-      const bool val = warp == 10;
-      const int32_t *table = p.c.table + i * p.c.table_stride;
-      const int mask = (1 << p.c.shift) - 1, gi = val ? lane : lane / Sm::kHalves, hf = val ? 0 : lane % Sm::kHalves;
-      auto page_of = [&](int j) {
-        const int g = j * kPpGroups + gi;
-        return j < j1 && gi < kPpGroups && g < sp.groups ? table[sp.slot(g) >> p.c.shift] : -1;
-      };
-      int page = page_of(j0), fill = val ? 1 : 0;
-      for (int j = j0; j < j1; ++j, fill += 2) {
-        const int next = page_of(j + 1);
-        const int ng = min(kPpGroups, sp.groups - j * kPpGroups);
-        const int slot = gi < ng ? sp.slot(j * kPpGroups + gi) : 0;
-        const int s = fill % ST;
-        if (fill >= ST) pp_wait(&empty[s], (fill / ST - 1) & 1, dead, 11);
-        if (*dead) break;
-        if (lane == 0) tc_expect_tx(&full[s], unsigned(ng * kPpGroup * HD * 2));
-        __syncwarp();
-        const uint32_t dst = tc_saddr(ring + s * Sm::kTile);
-        if (gi < ng) {
-          if (val) pp_tma_v(dst + gi * Sm::kVGroup, &vmap, slot & mask, h, page, &full[s]);
-          else pp_tma_k(dst + hf * kPpHalf + gi * (kPpGroup * 128), &kmap, hf * 64, slot & mask, h, page, &full[s]);
+    // One elected thread a warp issues. (Issued by `lane == 0` instead, an MMA took 480 clocks of its warp beside
+    // 16 busy ones, against 70: only elect.sync tells the compiler that one thread is left.)
+    if (warp == kWalk) {
+     if (tc_elect()) {
+      // the walk along the CTA's part, and Q
+      long long u = share.place, left = share.end - share.begin;
+      const long long places = (long long)p.c.seqs * p.blocks;
+      int off = share.off, h = share.head_len ? int(share.begin / share.head_len) : 0, nq = 0, k = 0;
+      PpHead head{};
+      for (;; ++k) {
+        PpSeg sg;
+        bool some = false;
+        while (left > 0 && !some) {
+          if (u >= places) {
+            u = 0;
+            ++h;
+          }
+          if (!pp_place(p, u, &sg)) {
+            u = (u / p.blocks + 1) * p.blocks;
+            continue;
+          }
+          const int nt = sg.tiles();
+          const int take = int(min(left, (long long)(nt + 1 - off)));
+          sg.i = int(u / p.blocks);
+          sg.h = h;
+          sg.j0 = min(off, nt);
+          sg.j1 = min(off + take, nt);
+          sg.part = sg.j0 == 0 && sg.j1 == nt ? -1 : 2 * int(blockIdx.x) + (sg.j0 == 0 ? 1 : 0);
+          some = sg.j1 > sg.j0 || nt == 0;
+          if (some && sg.j0 == 0 && sg.j1 < nt) {
+            const long long first = share.end - left;
+            head = PpHead{int((first + nt - 1) / share.part - blockIdx.x + 1), sg.row0, sg.t0, sg.t1, h, {0, 0, 0}};
+          }
+          left -= take;
+          off += take;
+          if (off > nt) {
+            off = 0;
+            ++u;
+          }
         }
-        page = next;
+        if (!some) sg.h = -1;
+        if (k >= kPpSegs) pp_wait(&segempty[k % kPpSegs], (k / kPpSegs - 1) & 1, dead, 12);
+        if (*dead) break;
+        segs[k % kPpSegs] = sg;
+        tc_arrive(&segfull[k % kPpSegs]);
+        if (!some) break;
+        if (sg.j1 > sg.j0) {
+          if (nq > 0) pp_wait(&qempty, (nq - 1) & 1, dead, 13);
+          if (*dead) break;
+          const int two = sg.t1 - sg.t0 > p.tokens ? 2 : 1;
+          tc_expect_tx(&qfull, unsigned(two * p.tokens * p.a.rep * HD * 2));
+          for (int x = 0; x < two; ++x)
+#pragma unroll
+            for (int hf = 0; hf < Sm::kHalves; ++hf)
+              pp_tma_k(tc_saddr(qsm + x * Sm::kTile + hf * kPpHalf), &qmap, hf * 64, 0, sg.h, sg.row0 + sg.t0 + x * p.tokens,
+                       &qfull);
+          ++nq;
+        }
+      }
+      if (gridDim.x > 1) p.heads[blockIdx.x] = head;
+      // after a wait that ran out: no copy may be in flight when the CTA ends
+      if (*dead && nq > 0) tc_wait(&qfull, (nq - 1) & 1, &pp_status_word, 14);
+     }
+    } else if (warp == kCopy) {
+      // K and V of each tile, in turn, a ring stage each. Rows of V that no row of the block sees are zeroed
+      // once they are there, by the whole warp; the MMAs hear of the stage after that.
+      const bool chosen = tc_elect();
+      const int mask = (1 << p.c.shift) - 1;
+      const int step = p.box / kPpGroup;          // groups of a box
+      int s = 0, turn = 0, lands = 0, fills = 0;  // the next stage, how often the ring has gone round
+      for (int k = 0;; ++k) {
+        const PpSeg &sg = seg_get(k);
+        if (__any_sync(0xffffffffu, *dead || sg.h < 0)) break;
+        const int32_t *table = p.c.table + sg.i * p.c.table_stride;
+        const int pmax = sg.p0 + sg.t1 - 1;
+        int page[kPpGroups];  // of the tile's boxes, read a tile ahead
+        auto pages_of = [&](int j) {
+#pragma unroll
+          for (int u = 0; u < kPpGroups; ++u) {
+            const int gg = j * kPpGroups + u * step;
+            page[u] = j < sg.j1 && u * step < kPpGroups && gg < sg.groups ? table[sg.slot(gg) >> p.c.shift] : -1;
+          }
+        };
+        auto take = [&]() {  // the next stage, free
+          if (turn > 0) pp_wait(&empty[s], (turn - 1) & 1, dead, 15);
+          ++fills;
+          return s;
+        };
+        auto next = [&]() {
+          if (++s == ST) {
+            s = 0;
+            ++turn;
+          }
+        };
+        auto copy_k = [&](int j) {
+          const int ng = min(kPpGroups, sg.groups - j * kPpGroups), at = take();
+          uint8_t *dst = ring + at * Sm::kTile;
+          if (chosen && !*dead) {
+            tc_expect_tx(&full[at], unsigned((ng + step - 1) / step * p.box * HD * 2));
+#pragma unroll
+            for (int u = 0; u < kPpGroups; ++u) {
+              const int g = u * step;
+              if (g >= ng) break;
+              const int row = sg.slot(j * kPpGroups + g) & mask;
+#pragma unroll
+              for (int hf = 0; hf < Sm::kHalves; ++hf)
+                pp_tma_k(tc_saddr(dst + hf * kPpHalf + g * (kPpGroup * 128)), &kmap, hf * 64, row, sg.h, page[u], &full[at]);
+            }
+          }
+          next();
+        };
+        pages_of(sg.j0);
+        if (sg.j0 < sg.j1) copy_k(sg.j0);
+        for (int j = sg.j0; j < sg.j1; ++j) {
+          const int gb = j * kPpGroups, ng = min(kPpGroups, sg.groups - gb);
+          const int jb = sg.slot(gb), je = sg.slot(gb + ng - 1) + kPpGroup;
+          const bool edge = !(je - 1 <= pmax && (jb >= sg.lo || je <= sg.first));
+          const int at = take();
+          uint8_t *dst = ring + at * Sm::kTile;
+          if (chosen && !*dead) {
+            uint64_t *bar = edge ? &vland : &full[at];
+            tc_expect_tx(bar, unsigned((ng + step - 1) / step * p.box * HD * 2));
+#pragma unroll
+            for (int u = 0; u < kPpGroups; ++u) {
+              const int g = u * step;
+              if (g >= ng) break;
+              pp_tma_v(tc_saddr(dst + g * (kPpGroup * HD * 2)), &vmap, sg.slot(gb + g) & mask, sg.h, page[u], bar);
+            }
+          }
+          next();
+          pages_of(j + 1);
+          if (j + 1 < sg.j1) copy_k(j + 1);
+          if (edge) {
+            pp_wait(&vland, lands++ & 1, dead, 26);
+            for (int g = 0; g < ng; ++g) {
+              const int s0 = sg.slot(gb + g);
+              if (s0 + kPpGroup - 1 <= pmax && (s0 >= sg.lo || s0 + kPpGroup <= sg.first)) continue;
+              for (int e = lane; e < kPpGroup * Sm::kHalves * 8; e += 32) {
+                const int r = e / (Sm::kHalves * 8), ch = e % (Sm::kHalves * 8), s1 = s0 + r;
+                if (s1 > pmax || (s1 < sg.lo && s1 >= sg.first))
+                  *reinterpret_cast<uint4 *>(dst + pp_voff<HD>(g * kPpGroup + r, ch >> 3, p.box) + (ch & 7) * 16) =
+                      make_uint4(0, 0, 0, 0);
+              }
+            }
+            tc_fence_proxy();
+            __syncwarp();
+            if (chosen) tc_arrive(&full[at]);
+          }
+          if (__any_sync(0xffffffffu, *dead)) break;
+        }
+        if (__any_sync(0xffffffffu, *dead)) break;
+        seg_done(k);
       }
       // after a wait that ran out: no copy may be in flight when the CTA ends
-      if (*dead)
-        for (int f = max(val ? 1 : 0, fill - 2 * ST); f < fill; f += 2)
-          tc_wait(&full[f % ST], (f / ST) & 1, &pp_status_word, 12);
-    } else if (warp == 9) {
+      if (__any_sync(0xffffffffu, *dead)) {
+        for (int f = max(0, fills - ST); f < fills; ++f) tc_wait(&full[f % ST], (f / ST) & 1, &pp_status_word, 16);
+        if (lands > 0) tc_wait(&vland, (lands - 1) & 1, &pp_status_word, 14);
+      }
+    } else if (tc_elect()) {
+      // The MMAs of tile A (warp kMma) or B (the next): a warp each, since a step's waits and commits take one
+      // thread about as long as its MMAs take the tensor cores.
+      const int x = warp - kMma;
+      const uint32_t ts = tmem + x * 128, to = tmem + 256 + x * 128;
       // descriptors of the first K-step; the others differ in the address (units of 16 bytes)
-      const uint64_t qd[2] = {pp_desc(tc_saddr(qsm), 16), pp_desc(tc_saddr(qsm) + Sm::kTile, 16)};
-      const uint64_t kd = pp_desc(tc_saddr(ring), 16), vd = pp_desc(tc_saddr(ring), Sm::kVHalf);
+      const uint64_t qd = pp_desc(tc_saddr(qsm + x * Sm::kTile), 16);
+      const uint64_t kd = pp_desc(tc_saddr(ring), 16), vd = pp_desc(tc_saddr(ring), p.box * 128);
       const uint32_t idv = pp_idesc(BF, HD, true);
-      auto scores = [&](int x, int s, int ng) {  // S_x = Q_x K^T of the stage's ng groups
-        const uint32_t id = pp_idesc(BF, ng * kPpGroup, false);
-        const uint64_t kb = kd + s * (Sm::kTile >> 4);
+      const uint32_t neg = p.a.scale < 0.f ? 1u << 13 : 0u;  // the softmax takes |scale|
+      const uint32_t idk = pp_idesc(BF, 0, false) | neg;
+      auto scores = [&](int at, int ng) {  // S = +-Q K^T of the stage's ng groups
+        const uint64_t kb = kd + at * (Sm::kTile >> 4);
+        const uint32_t id = idk | uint32_t(ng * (kPpGroup >> 3)) << 17;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t off = ((k >> 2) * kPpHalf + (k & 3) * 32) >> 4;
-          tc_mma(tmem + x * 128, qd[x] + off, kb + off, id, k > 0);
+          tc_mma(ts, qd + off, kb + off, id, k > 0);
         }
-        tc_commit(&sfull[x]);
       };
-      auto values = [&](int x, int s, int ng, bool add) {  // O_x += P_x V
-        const uint64_t vb = vd + s * (Sm::kTile >> 4);
+      uint32_t vo[kPpGroups];  // V's groups in a stage, in units of 16 bytes
 #pragma unroll
-        for (int k = 0; k < kPpGroups; ++k)
-          if (k < ng)
-            pp_mma_ta(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, vb + k * (Sm::kVGroup >> 4), idv, add || k > 0);
-        tc_commit(&ofull[x]);
+      for (int g = 0; g < kPpGroups; ++g) vo[g] = pp_voff<HD>(g * kPpGroup, 0, p.box) >> 4;
+      auto values = [&](int at, int half, int ng, int add) {  // O += P V of a half's groups, as far as there are ng
+        const uint64_t vb = vd + at * (Sm::kTile >> 4);
+        if (half == 0) {
+#pragma unroll
+          for (int k = 0; k < kPpGroups / 2; ++k)
+            if (k < ng) pp_mma_ta(to, ts + 8 * k, vb + vo[k], idv, k > 0 ? 1 : add);
+        } else {
+#pragma unroll
+          for (int k = kPpGroups / 2; k < kPpGroups; ++k)
+            if (k < ng) pp_mma_ta(to, ts + 8 * k, vb + vo[k], idv, 1);
+        }
       };
-      auto groups_of = [&](int j) { return min(kPpGroups, sp.groups - j * kPpGroups); };
-      const int n = j1 - j0;
-      if (n > 0) {
-        pp_wait(&qfull, 0, dead, 13);
-        pp_wait(&full[0], 0, dead, 14);
+      int s = 0, turn = 0;  // the ring, as the copying warp fills it
+      auto next = [&]() {
+        if (++s == ST) {
+          s = 0;
+          turn ^= 1;
+        }
+      };
+      int nq = 0, step = 0, blocks = 0;
+      for (int k = 0;; ++k) {
+        const PpSeg &sg = seg_get(k);
+        if (*dead || sg.h < 0) break;
+        const int n = sg.j1 - sg.j0;
+        int left = sg.groups - sg.j0 * kPpGroups;  // groups from this tile on
+        const bool two = sg.t1 - sg.t0 > p.tokens;
+        tc_arrive(&segempty[k % kPpSegs]);
+        if (n <= 0) continue;
+        ++nq;
+        if (x == 1 && !two) {  // tile B has no rows: its part of the stages' release
+          for (int v = 0; v < 2 * n; ++v, next()) {
+            pp_wait(&full[s], turn, dead, 19);
+            tc_arrive(&empty[s]);
+          }
+          pp_wait(&qfull, (nq - 1) & 1, dead, 17);  // no further ahead of A than a block
+          tc_arrive(&qempty);
+          continue;
+        }
+        pp_wait(&qfull, (nq - 1) & 1, dead, 17);
+        pp_wait(&full[s], turn, dead, 18);
         tc_fence_after();
-        if (lane == 0) {
-          scores(0, 0, groups_of(j0));
-          if (two) scores(1, 0, groups_of(j0));
-          tc_commit(&empty[0]);
-        }
-      }
-      const int pmax = sp.p0 + sp.t1 - 1;
-      for (int u = 0; u < n; ++u) {
-        const int j = j0 + u, ng = groups_of(j), fv = 2 * u + 1, fk = 2 * u + 2;
-        pp_wait(&full[fv % ST], (fv / ST) & 1, dead, 15);
-        // values of slots that no row of this CTA sees
-        const int jb = sp.slot(j * kPpGroups), je = sp.slot(j * kPpGroups + ng - 1) + kPpGroup;
-        if (je - 1 > pmax || (jb < sp.lo && je > sp.first)) {
-          for (int g = 0; g < ng; ++g) {
-            const int s0 = sp.slot(j * kPpGroups + g);
-            if (s0 + kPpGroup - 1 <= pmax && (s0 >= sp.lo || s0 + kPpGroup <= sp.first)) continue;
-            for (int e = lane; e < kPpGroup * Sm::kHalves * 8; e += 32) {
-              const int r = e / (Sm::kHalves * 8), ch = e % (Sm::kHalves * 8), s = s0 + r;
-              if (s > pmax || (s < sp.lo && s >= sp.first))
-                *reinterpret_cast<uint4 *>(ring + (fv % ST) * Sm::kTile + g * Sm::kVGroup + (ch >> 3) * Sm::kVHalf +
-                                           r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          tc_fence_proxy();
-        }
-        if (u + 1 < n) pp_wait(&full[fk % ST], (fk / ST) & 1, dead, 16);
-        __syncwarp();
-        for (int x = 0; x < (two ? 2 : 1); ++x) {
-          pp_wait(&pfull[x], u & 1, dead, 17);
+        scores(s, min(kPpGroups, left));
+        tc_commit(&sfull[x]);
+        tc_commit(&empty[s]);
+        if (n == 1) tc_commit(&qempty);
+        next();
+        for (int v = 0; v < n; ++v, ++step) {
+          const int sv = s;
+          pp_wait(&full[sv], turn, dead, 19);
+          if (v == 0 && blocks > 0) pp_wait(&ofree[x], (blocks - 1) & 1, dead, 20);
+          pp_wait(&pfull[x][0], step & 1, dead, 21);
           tc_fence_after();
-          if (lane == 0) {
-            values(x, fv % ST, ng, u > 0);
-            if (u + 1 < n) scores(x, fk % ST, groups_of(j + 1));
+          values(sv, 0, left, v > 0);
+          pp_wait(&pfull[x][1], step & 1, dead, 28);
+          tc_fence_after();
+          values(sv, 1, left, 1);
+          next();
+          left -= kPpGroups;
+          if (v + 1 < n) {
+            pp_wait(&full[s], turn, dead, 23);
+            scores(s, min(kPpGroups, left));
+            tc_commit(&sfull[x]);
+            tc_commit(&empty[sv]);
+            tc_commit(&empty[s]);
+            if (v + 2 == n) tc_commit(&qempty);
+            next();
+          } else {
+            tc_commit(&ofull[x]);
+            tc_commit(&empty[sv]);
           }
+          if (*dead) break;
         }
-        if (lane == 0) {
-          tc_commit(&empty[fv % ST]);
-          if (u + 1 < n) tc_commit(&empty[fk % ST]);
-        }
+        ++blocks;
+        if (*dead) break;
       }
-      if (lane == 0) {
-        tc_commit(&done);
-        tc_wait(&done, 0, &pp_status_word, 18);
-      }
-      __syncwarp();
+      tc_commit(&done[x]);
+      tc_wait(&done[x], 0, &pp_status_word, 25);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpSoftRegs));
-    if (warp < 4 || two) {
-      const int x = warp >> 2, row = threadIdx.x & 127;
-      pp_load_q<HD>(p, sp, h, sp.t0 + x * p.tokens, qsm + x * Sm::kTile, row);
-      tc_fence_proxy();
-      __syncwarp();
-      if (lane == 0) tc_arrive(&qfull);
-      // this thread's row: token t of the sequence, query head hq
-      const int rt = row / p.a.rep, t = sp.t0 + x * p.tokens + rt, hq = h * p.a.rep + row % p.a.rep;
-      const bool mine = rt < p.tokens && t < sp.t1;
-      const int pos = mine ? sp.p0 + t : -1;
-      const int wlo = p.a.window > 0 ? pos - p.a.window + 1 : -(1 << 30);  // the first slot in the window
-      const float scale2 = fmaxf(fabsf(p.a.scale) * kPpLog2e, 1e-37f);
-      constexpr float kBias = BF ? 0.f : 7.f;
-      const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-      const uint32_t ts = tmem + x * 128 + lanes, to = tmem + 256 + x * 128 + lanes;
-      const int pmin = sp.p0 + sp.t0, pmax = sp.p0 + sp.t1 - 1;
+    const int x = warp >> 2, row = threadIdx.x & 127;
+    // row / rep of a row below 128, rep at most 128: 65,536 / rep rounded up is close enough to be exact
+    const int rep = p.a.rep, recip = (65536 + rep - 1) / rep;
+    auto token_of = [&](int r) { return (r * recip) >> 16; };
+    const int rt = token_of(row);  // this thread's token of the tile
+    const float scale2 = fmaxf(fabsf(p.a.scale) * kPpLog2e, 1e-37f);
+    constexpr float kBias = BF ? 0.f : 7.f;
+    const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
+    const uint32_t ts = tmem + x * 128 + lanes, to = tmem + 256 + x * 128 + lanes;
+    int step = 0, done_blocks = 0, turns = 0;  // tiles, blocks and turns so far
+    for (int k = 0;; ++k) {
+      const PpSeg &sg = seg_get(k);
+      if (__any_sync(0xffffffffu, *dead || sg.h < 0)) break;
+      const int tok0 = sg.t0 + x * p.tokens, left = min(p.tokens, sg.t1 - tok0);  // the tile's tokens
+      if (left <= 0) {  // tile B has no rows
+        seg_done(k);
+        continue;
+      }
+      const int pmin = sg.p0 + sg.t0, pmax = sg.p0 + sg.t1 - 1, n = sg.j1 - sg.j0, g0 = sg.j0 * kPpGroups;
+      // of this row: its slot (before all of them for a row that is none) and the first slot in the window; of the
+      // block's last row the latter, too
+      const int pos = rt < left ? sg.p0 + tok0 + rt : -1;
+      const bool windowed = p.a.window > 0;
+      const int wlo = windowed ? pos - p.a.window + 1 : -(1 << 30), wmax = windowed ? pmax - p.a.window + 1 : -(1 << 30);
+      const int ga = sg.ga, b0 = sg.b0 - sg.ga, groups = sg.groups;
+      // The exponentials of the two tiles take turns, warp by warp (warps w and w + 4 share a scheduler): side by
+      // side they take twice as long each, and then both tiles wait for MMAs at the same time (575 us against
+      // 549 for the 16,384-token prompt). Blocks of few tiles end before that pays (257 us against 294 for
+      // ragged prompts in a window of 128).
+      const bool alternate = sg.t1 - sg.t0 > p.tokens && n >= kPpGroups;
+      // groups [whole0, whole1) are seen by every row of the block: slots from wmax to pmin, in one run
+      const int whole0 = max(b0 > 0 ? ga : 0, (max(wmax, 0) + kPpGroup - 1) / kPpGroup - b0);
+      const int whole1 = (pmin + 1) / kPpGroup - b0;
       float m = -INFINITY, ref = 0.f, l = 0.f;  // m: of the scores as they are; ref: of exp2's argument
-      for (int u = 0; u < j1 - j0; ++u) {
-        const int gb = (j0 + u) * kPpGroups, ng = min(kPpGroups, sp.groups - gb);
-        pp_wait(&sfull[x], u & 1, dead, 19);
+      for (int v = 0; v < n; ++v, ++step) {
+        const int gb = g0 + v * kPpGroups;
+        const bool half_only = groups - gb <= kPpGroups / 2;  // a last tile with no more than a half
+        pp_wait(&sfull[x], step & 1, dead, 24);
         tc_fence_after();
+        if (!(gb >= whole0 && gb + kPpGroups <= whole1)) {
+          // hidden scores, in tensor memory, a group at a time (a short loop: straight code for 128 columns was
+          // fetched anew for every block); groups that all rows of the block see are left alone
+#pragma unroll 1
+          for (int g = 0; g < (half_only ? kPpGroups / 2 : kPpGroups); ++g) {
+            const int gg = gb + g, s0 = gg < groups ? kPpGroup * (gg < ga ? gg : gg + b0) : (1 << 30);
+            if (s0 + kPpGroup - 1 <= pmin && (s0 >= wmax || s0 + kPpGroup <= p.a.first)) continue;
+            // the visible columns of the group: c <= hi and (c >= lo or c < fi)
+            const int hi = min(max(pos - s0 + 1, 0), 16), lo = min(max(wlo - s0, 0), 16);
+            const int fi = min(max(p.a.first - s0, 0), 16);
+            const uint32_t see = ((1u << hi) - 1) & (~((1u << lo) - 1) | ((1u << fi) - 1));
+            float y[16];
+            uint32_t z[16];
+            tc_ld16(ts + 16 * g, y);
+#pragma unroll
+            for (int c = 0; c < kPpGroup; ++c) z[c] = (see & (1u << c)) ? __float_as_uint(y[c]) : 0xff800000u;
+            pp_st16(ts + 16 * g, z);
+          }
+          pp_wait_st();
+        }
         uint32_t s[128];
         pp_ld128(ts, s);
-        const int jb = sp.slot(gb), je = sp.slot(gb + ng - 1) + kPpGroup;
-        const bool whole = ng == kPpGroups && je - jb == kPpSlots && je - 1 <= pmin &&
-                           (p.a.window == 0 || jb > pmax - p.a.window || je <= p.a.first);
-        if (!whole) {
+        if (half_only) {
 #pragma unroll
-          for (int g = 0; g < kPpGroups; ++g) {
-            const int s0 = g < ng ? sp.slot(gb + g) : (1 << 30);
-            const int hi = pos - s0, lo = wlo - s0, fi = p.a.first - s0;  // column c: c <= hi and (c >= lo or c < fi)
-#pragma unroll
-            for (int c = 0; c < kPpGroup; ++c)
-              if (!(c <= hi && (c >= lo || c < fi))) s[g * kPpGroup + c] = 0xff800000u;
-          }
+          for (int c = 64; c < kPpSlots; ++c) s[c] = 0xff800000u;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < kPpSlots; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const bool move = (top - m) * scale2 > kPpLazy || (m == -INFINITY && top > m);
+        for (int c = 0; c < kPpSlots; c += 2)
+          mx[(c >> 1) & 3] = pp_max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        const float top = fmaxf(pp_max3(mx[0], mx[1], mx[2]), mx[3]);
+        const bool move = (top - m) * scale2 > kPpLazy;
         if (__any_sync(0xffffffffu, move)) {
           float f = 1.f;
           if (move) {
@@ -474,120 +785,164 @@ __global__ void __launch_bounds__(kPpThreads, 1)
             ref = nref;
             l *= f;
           }
-          if (u > 0) {
-            pp_wait(&ofull[x], (u - 1) & 1, dead, 20);
-            tc_fence_after();
+          if (v > 0) {
+            // O is complete up to the last tile: these scores were issued behind its product
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              float o[16];
+              uint32_t w[16];
+              tc_ld16(to + c, o);
 #pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-              uint32_t o[32];
-              pp_ld32(to + c, o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              pp_st32(to + c, o);
+              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
+              pp_st16(to + c, w);
             }
           }
         }
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        if (alternate) {
+          if (x == 1) pp_wait(&exp_turn[1][warp & 3], turns & 1, dead, 29);
+          else if (turns > 0) pp_wait(&exp_turn[0][warp & 3], (turns - 1) & 1, dead, 29);
+          ++turns;
+        }
+        uint64_t ls[2] = {0, 0};
+        const uint64_t sc2 = pp_two(scale2, scale2), rf2 = pp_two(-ref, -ref);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const float a = pp_exp2(fmaf(__uint_as_float(s[64 * half + c]), scale2, -ref));
-            const float b = pp_exp2(fmaf(__uint_as_float(s[64 * half + c + 1]), scale2, -ref));
-            ls[c & 2] += a;
-            ls[(c & 2) + 1] += b;
-            pk[c / 2] = pp_pack<BF>(a, b);
+          if (half == 1 && half_only) {
+            if (lane == 0) tc_arrive(&pfull[x][1]);
+            break;
           }
-          pp_st32(ts + 32 * half, pk);
+          uint32_t w[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const uint64_t x2 =
+                pp_fma2(pp_two(__uint_as_float(s[64 * half + 2 * c]), __uint_as_float(s[64 * half + 2 * c + 1])), sc2, rf2);
+            float2 e = pp_split(x2);
+            e.x = pp_exp2(e.x);
+            e.y = pp_exp2(e.y);
+            ls[c & 1] = pp_add2(ls[c & 1], pp_two(e.x, e.y));
+            w[c] = pp_pack<BF>(e.x, e.y);
+          }
+          pp_st32(ts + 32 * half, w);
+          pp_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc_arrive(&pfull[x][half]);
         }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        pp_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc_arrive(&pfull[x]);
+        if (alternate && lane == 0) tc_arrive(&exp_turn[x ^ 1][warp & 3]);
+        const float2 lsum = pp_split(pp_add2(ls[0], ls[1]));
+        l += lsum.x + lsum.y;
       }
-      if (j1 > j0) {
-        pp_wait(&ofull[x], (j1 - j0 - 1) & 1, dead, 21);
+      // The rows: O / l, or what a second kernel makes it of. O is read as an MMA's fragment, 16 rows and 32
+      // columns at a time, and a quad's words are transposed, so that rows leave in runs of 64 bytes.
+      const int part = sg.part, hq0 = sg.h * rep;
+      float f = 1.f;
+      if (part < 0) {
+        if (p.a.sinks && pos >= 0) l += pp_exp2(p.a.sinks[hq0 + row - rt * rep] * kPpLog2e - ref);
+        f = m > -INFINITY ? 1.f / l : 0.f;  // zeros for a row that sees nothing
+      } else if (rt < left) {
+        p.part_ml[int64_t(part) * p.slot_rows + x * p.tokens * rep + row] = make_float2(m == -INFINITY ? -INFINITY : ref, l);
+      }
+      if (n > 0) {
+        pp_wait(&ofull[x], done_blocks & 1, dead, 27);
+        ++done_blocks;
         tc_fence_after();
       }
-      float inv = 1.f;
-      const int64_t at = (int64_t(sp.row0 + t) * p.a.heads + hq) * p.splits + split;
-      if (alone) {
-        if (p.a.sinks && mine) l += pp_exp2(p.a.sinks[hq] * kPpLog2e - ref);
-        inv = l > 0.f ? 1.f / l : 0.f;
-      } else if (mine) {
-        *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(m == -INFINITY ? -INFINITY : ref, l);
-      }
-      uint16_t *out = p.a.o + int64_t(sp.row0 + t) * p.a.o_row + hq * p.a.o_head;
-#pragma unroll
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
-        if (j1 > j0) {
-          pp_ld32(to + c, o);
+      const int q = lane & 3;
+      uint16_t *out0 = p.a.o + int64_t(sg.row0 + tok0) * p.a.o_row + hq0 * p.a.o_head + 8 * q;
+      float *part0 = p.part_o + (int64_t(part) * p.slot_rows + x * p.tokens * rep) * HD + 2 * q;
+#pragma unroll 1
+      for (int u = 0; u < HD / 16; ++u) {
+        const int r16 = 16 * (u & 1), col = 32 * (u >> 1);
+        uint32_t o[16];
+        if (n > 0) {
+          pp_ldo(to + (uint32_t(r16) << 16) + col, o);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+          for (int e = 0; e < 16; ++e) o[e] = 0u;
         }
-        if (!mine) continue;
-        if (alone) {
+        if (u == HD / 16 - 1 && n > 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc_arrive(&ofree[x]);
+        }
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 v;
-            v.x = pp_pack<BF>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-            v.y = pp_pack<BF>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-            v.z = pp_pack<BF>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-            v.w = pp_pack<BF>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-            *reinterpret_cast<uint4 *>(out + c + e) = v;
+        for (int b = 0; b < 2; ++b) {
+          const int lr = r16 + 8 * b + (lane >> 2), rr = 32 * (warp & 3) + lr;  // the row in the warp, in the tile
+          const float fr = __shfl_sync(0xffffffffu, f, lr);
+          const int tt = token_of(rr);
+          if (part < 0) {
+            // words of column blocks i; the quad's 4 x 4 words are transposed: lane q gets block q
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = pp_pack<BF>(__uint_as_float(o[4 * i + 2 * b]) * fr, __uint_as_float(o[4 * i + 2 * b + 1]) * fr);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 1) ? w[i] : w[i + 1], 1);
+              if (q & 1) w[i] = got;
+              else w[i + 1] = got;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 2) ? w[i] : w[i + 2], 2);
+              if (q & 2) w[i] = got;
+              else w[i + 2] = got;
+            }
+            uint16_t *out = out0 + tt * p.a.o_row + (rr - tt * rep) * p.a.o_head + col;
+            if (tt < left) *reinterpret_cast<uint4 *>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else if (tt < left) {
+            float *out = part0 + int64_t(rr) * HD + col;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint2 *>(out + 8 * i) = make_uint2(o[4 * i + 2 * b], o[4 * i + 2 * b + 1]);
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4 *>(p.part_o + at * HD + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       }
+      seg_done(k);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMma) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPpTmem) : "memory");
   }
 }
 
-// Joins the splits of a token's query heads, a warp a head.
+constexpr int kPpJoinRows = 16;  // rows a CTA of the joining kernel takes, a warp a row
+
+// Joins the parts of the block that CTA blockIdx.x began and others went on with, in order.
 template <int HD, bool BF>
 __global__ void __launch_bounds__(128) paged_prompt_join_kernel(const PpArgs p) {
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x, i = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  PpSpan sp;
-  if (!sp.set(p.c, p.a, p.starts, p.rows, p.max_rows, i, 2 * p.tokens, t / (2 * p.tokens)) || t >= sp.t1) return;
-  const int per = sp.per(p.splits), used = (sp.tiles() + per - 1) / per;
-  if (used <= 1) return;  // the first kernel wrote it
+  const PpHead hd = p.heads[blockIdx.x];
+  if (hd.parts <= 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int E = HD / 32;
-  for (int hq = warp; hq < p.a.heads; hq += 4) {
-    const int64_t at = (int64_t(sp.row0 + t) * p.a.heads + hq) * p.splits;
+  for (int r = blockIdx.y * kPpJoinRows + warp; r < (int(blockIdx.y) + 1) * kPpJoinRows; r += 4) {
+    const int t = hd.t0 + r / p.a.rep, hq = hd.h * p.a.rep + r % p.a.rep;
+    if (t >= hd.t1) return;
+    // the first part is what its CTA ended with, the others what theirs began with
+    auto at = [&](int s) { return int64_t(2 * (blockIdx.x + s) + (s == 0 ? 1 : 0)) * p.slot_rows + r; };
     const float sink = p.a.sinks ? p.a.sinks[hq] * kPpLog2e : -INFINITY;
     float m = sink;
-    for (int s = lane; s < used; s += 32) m = fmaxf(m, p.part_ml[2 * (at + s)]);
+    for (int s = lane; s < hd.parts; s += 32) m = fmaxf(m, p.part_ml[at(s)].x);
     m = warp_max(m);
     const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int s = lane; s < used; s += 32) l += exp2f(p.part_ml[2 * (at + s)] - ref) * p.part_ml[2 * (at + s) + 1];
-    l = warp_sum(l) + exp2f(sink - ref);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    float v[E];
+    float l = exp2f(sink - ref), v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < used; ++s) {
-      const float f = exp2f(p.part_ml[2 * (at + s)] - ref);
+    for (int s = 0; s < hd.parts; ++s) {
+      const float2 ml = p.part_ml[at(s)];
+      const float f = exp2f(ml.x - ref);
+      l = fmaf(f, ml.y, l);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = fmaf(f, p.part_o[(at + s) * HD + lane * E + e], v[e]);
+      for (int e = 0; e < E; ++e) v[e] = fmaf(f, p.part_o[at(s) * HD + lane * E + e], v[e]);
     }
-    uint16_t *out = p.a.o + int64_t(sp.row0 + t) * p.a.o_row + hq * p.a.o_head + lane * E;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint16_t *out = p.a.o + int64_t(hd.row0 + t) * p.a.o_row + hq * p.a.o_head + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(out + e) = pp_pack<BF>(v[e] * inv, v[e + 1] * inv);
   }
@@ -612,10 +967,10 @@ EncodeFn pp_encoder() {
   return reinterpret_cast<EncodeFn>(f);
 }
 
-// The pool as (column, row of a page, head, page), a box of 16 rows x 64 columns (K), or as (column of a
-// half, row, half, head, page), a box of 16 rows x all columns, half by half (V); 128-byte swizzle, and
+// The pool as (column, row of a page, head, page), a box of `box` rows x 64 columns (K), or as (column of a
+// half, row, half, head, page), a box of `box` rows x all columns, half by half (V); 128-byte swizzle, and
 // what lies outside reads as zeros.
-bool pp_map(EncodeFn enc, const PagedView &c, bool halves, CUtensorMap *map) {
+bool pp_kv_map(EncodeFn enc, const PagedView &c, bool halves, int box, CUtensorMap *map) {
   const cuuint64_t row = cuuint64_t(c.row_stride) * 2;
   // a dimension of one has no stride of its own
   const cuuint64_t head = c.kv_heads > 1 ? cuuint64_t(c.head_stride) * 2 : row;
@@ -623,7 +978,7 @@ bool pp_map(EncodeFn enc, const PagedView &c, bool halves, CUtensorMap *map) {
   const cuuint64_t rows = cuuint64_t(1) << c.shift, heads = cuuint64_t(c.kv_heads), pages = cuuint64_t(c.pages);
   const cuuint64_t kdims[4] = {cuuint64_t(c.hd), rows, heads, pages}, kstr[3] = {row, head, page};
   const cuuint64_t vdims[5] = {64, rows, cuuint64_t(c.hd / 64), heads, pages}, vstr[4] = {row, 128, head, page};
-  const cuuint32_t kbox[4] = {64, kPpGroup, 1, 1}, vbox[5] = {64, kPpGroup, cuuint32_t(c.hd / 64), 1, 1};
+  const cuuint32_t kbox[4] = {64, cuuint32_t(box), 1, 1}, vbox[5] = {64, cuuint32_t(box), cuuint32_t(c.hd / 64), 1, 1};
   const cuuint32_t step[5] = {1, 1, 1, 1, 1};
   return enc(map, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, halves ? 5 : 4,
              halves ? c.v : c.k, halves ? vdims : kdims, halves ? vstr : kstr, halves ? vbox : kbox, step,
@@ -631,52 +986,63 @@ bool pp_map(EncodeFn enc, const PagedView &c, bool halves, CUtensorMap *map) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// q as (column, query head of a kv head, kv head, row), a box of 64 columns x rep heads x `tokens` rows.
+bool pp_q_map(EncodeFn enc, const PagedView &c, const PagedQuery &a, int rows, int tokens, CUtensorMap *map) {
+  const cuuint64_t head = a.heads > 1 ? cuuint64_t(a.q_head) * 2 : 16, row = rows > 1 ? cuuint64_t(a.q_row) * 2 : 16;
+  const cuuint64_t dims[4] = {cuuint64_t(c.hd), cuuint64_t(a.rep), cuuint64_t(c.kv_heads), cuuint64_t(rows)};
+  const cuuint64_t strides[3] = {head, head * a.rep, row};
+  const cuuint32_t box[4] = {64, cuuint32_t(a.rep), 1, cuuint32_t(tokens)}, step[4] = {1, 1, 1, 1};
+  return enc(map, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+             const_cast<uint16_t *>(a.q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // How a call is cut: by sizes alone, so that its scratch can be asked for beforehand.
 struct PpPlan {
-  int tokens, blocks, splits;
-  size_t ml, po;  // bytes
+  int tokens, blocks, ctas, slot_rows, box;
+  size_t heads_bytes, ml, po;
 };
 
 PpPlan pp_plan(const PagedView &c, int heads, int window, int first, int rows, int max_rows, int max_len, int sms) {
   PpPlan p{};
   if (rows < 1 || max_rows < 1) return p;
-  const int most = std::min(rows, max_rows);
-  p.tokens = kPpRows / (heads / c.kv_heads);
+  const int most = std::min(rows, max_rows), rep = heads / c.kv_heads;
+  p.tokens = kPpRows / rep;
   p.blocks = (most + 2 * p.tokens - 1) / (2 * p.tokens);
-  // The number of splits that ends soonest: waves of CTAs over the SMs times the tiles a CTA walks, with
-  // a CTA's start and end counted as kFixed tiles, and the second kernel as as many.
-  constexpr int kFixed = 4;
+  p.slot_rows = std::min(2 * p.tokens, most) * rep;
+  // The larger a TMA box, the fewer: a box costs about 100 clocks beside its bytes, and 64 KB a tile in boxes of
+  // 16 rows (24 of them) took 4,350 clocks, of 32 rows 3,180. But a window's first box begins up to box - 1 slots
+  // before it, so short windows take small ones.
+  p.box = kPpGroup;
+  while (p.box < kPpSlots && 2 * p.box <= (1 << c.shift) && (window == 0 || 16 * p.box <= window)) p.box *= 2;
+  // one CTA an SM, or fewer when the longest line the sizes allow has fewer parts of kPpMinPart tiles
   int64_t see = max_len;
-  if (window > 0) see = std::min<int64_t>(see, int64_t(window) + first + std::min(most, 2 * p.tokens));
-  const int64_t tiles = std::max<int64_t>(1, (see + kPpSlots - 1) / kPpSlots);
-  const int64_t units = int64_t(p.blocks) * c.kv_heads * c.seqs;
-  int64_t best = -1;
-  p.splits = 1;
-  for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
-    const int64_t per = (tiles + s - 1) / s;
-    if ((tiles + per - 1) / per != s) continue;
-    const int64_t cost = (units * s + sms - 1) / sms * (per + kFixed) + (s > 1 ? kFixed : 0);
-    if (best < 0 || cost < best) {
-      best = cost;
-      p.splits = int(s);
-    }
-  }
-  if (p.splits > 1) {
-    p.ml = (size_t(rows) * heads * p.splits * 2 * sizeof(float) + 255) / 256 * 256;
-    p.po = size_t(rows) * heads * p.splits * c.hd * sizeof(float);
+  if (window > 0) see = std::min<int64_t>(see, int64_t(window) + first + 2 * p.tokens + 2 * p.box);
+  const int64_t tiles = (see + kPpSlots - 1) / kPpSlots + 1;
+  const double line = double(p.blocks) * c.kv_heads * c.seqs * double(tiles);
+  p.ctas = int(std::max(1.0, std::min(double(sms), line / kPpMinPart + 1.0)));
+  if (p.ctas > 1) {
+    p.heads_bytes = (size_t(p.ctas) * sizeof(PpHead) + 255) / 256 * 256;
+    p.ml = (size_t(2) * p.ctas * p.slot_rows * sizeof(float2) + 255) / 256 * 256;
+    p.po = size_t(2) * p.ctas * p.slot_rows * c.hd * sizeof(float);
   }
   return p;
 }
 
+struct PpMaps {
+  CUtensorMap k, v, q;
+};
+
 template <int HD, bool BF>
-cudaError_t pp_launch(const PpArgs &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t st) {
+cudaError_t pp_launch(const PpArgs &p, const PpPlan &plan, const PpMaps &m, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(paged_prompt_kernel<HD, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        PpSmem<HD>::kBytes);
   if (e != cudaSuccess) return e;
-  launch_pdl(paged_prompt_kernel<HD, BF>, dim3(unsigned(p.blocks) * p.splits, p.c.kv_heads, p.c.seqs), dim3(kPpThreads),
-             PpSmem<HD>::kBytes, st, p, km, vm);
-  if (p.splits > 1)
-    launch_pdl(paged_prompt_join_kernel<HD, BF>, dim3(p.max_rows, p.c.seqs), dim3(128), 0, st, p);
+  launch_pdl(paged_prompt_kernel<HD, BF>, dim3(plan.ctas), dim3(kPpThreads), PpSmem<HD>::kBytes, st, p, m.k, m.v, m.q);
+  if (plan.ctas > 1)
+    launch_pdl(paged_prompt_join_kernel<HD, BF>, dim3(plan.ctas, (plan.slot_rows + kPpJoinRows - 1) / kPpJoinRows),
+               dim3(128), 0, st, p);
   return cudaGetLastError();
 }
 
@@ -692,7 +1058,7 @@ int paged_status_take() {
 size_t paged_prompt_scratch(const PagedView &c, int heads, int window, int first, int rows, int max_rows, int max_len,
                             int sms) {
   const PpPlan p = pp_plan(c, heads, window, first, rows, max_rows, max_len, sms);
-  return p.ml + p.po;
+  return p.heads_bytes + p.ml + p.po;
 }
 
 cudaError_t paged_prompt(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows, int max_rows,
@@ -700,13 +1066,16 @@ cudaError_t paged_prompt(const PagedView &c, const PagedQuery &a, const int32_t 
   const PpPlan plan = pp_plan(c, a.heads, a.window, a.first, rows, max_rows, max_len, sms);
   EncodeFn enc = pp_encoder();
   if (!enc) return cudaErrorNotSupported;
-  CUtensorMap km, vm;
-  if (!pp_map(enc, c, false, &km) || !pp_map(enc, c, true, &vm)) return cudaErrorInvalidValue;
+  PpMaps maps;
+  if (!pp_kv_map(enc, c, false, plan.box, &maps.k) || !pp_kv_map(enc, c, true, plan.box, &maps.v) || !pp_q_map(enc, c, a, rows, plan.tokens, &maps.q))
+    return cudaErrorInvalidValue;
   uint8_t *base = static_cast<uint8_t *>(scratch);
-  const PpArgs p{c, a, starts, rows, max_rows, plan.tokens, plan.blocks, plan.splits, reinterpret_cast<float *>(base),
-                 reinterpret_cast<float *>(base + plan.ml)};
-  if (c.hd == 128) return c.bf16 ? pp_launch<128, true>(p, km, vm, st) : pp_launch<128, false>(p, km, vm, st);
-  return c.bf16 ? pp_launch<64, true>(p, km, vm, st) : pp_launch<64, false>(p, km, vm, st);
+  const PpArgs p{c, a, starts, rows, max_rows, plan.tokens, plan.blocks, plan.slot_rows, plan.box,
+                 reinterpret_cast<PpHead *>(base),
+                 reinterpret_cast<float2 *>(base + plan.heads_bytes),
+                 reinterpret_cast<float *>(base + plan.heads_bytes + plan.ml)};
+  if (c.hd == 128) return c.bf16 ? pp_launch<128, true>(p, plan, maps, st) : pp_launch<128, false>(p, plan, maps, st);
+  return c.bf16 ? pp_launch<64, true>(p, plan, maps, st) : pp_launch<64, false>(p, plan, maps, st);
 }
 
 }  // namespace hc

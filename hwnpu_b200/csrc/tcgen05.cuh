@@ -47,6 +47,12 @@ __device__ __forceinline__ void tc_wait(uint64_t *b, unsigned parity, int *statu
     }
   }
 }
+// True on one thread of a converged warp.
+__device__ __forceinline__ bool tc_elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void tc_bulk(void *dst, const void *src, unsigned bytes, uint64_t *bar) {
   asm volatile(
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc_saddr(dst)),
