@@ -48,8 +48,8 @@ cudaError_t paged_append(const PagedView &c, const uint16_t *k, const uint16_t *
                          int64_t v_row, int64_t v_head, const int32_t *seq, const int32_t *slot, int rows,
                          cudaStream_t st);
 // idx: [seqs][kv_heads][keep] int32, the slots kept (-1 past the new length).
-cudaError_t paged_evict(const PagedView &c, const PagedView &to, int keep, int first, int recent, int32_t *idx,
-                        cudaStream_t st);
+cudaError_t paged_evict(const PagedView &c, const PagedView &to, int keep, int first, int recent, int max_len,
+                        int32_t *idx, cudaStream_t st);
 size_t paged_decode_scratch(const PagedView &c, int heads, int window, int first, int max_len, bool accumulate, int sms);
 cudaError_t paged_decode(const PagedView &c, const PagedQuery &a, int max_len, bool accumulate, void *scratch, int sms,
                          cudaStream_t st);

@@ -40,6 +40,7 @@ namespace {
 constexpr int kPdWarps = 4;
 constexpr int kPdGroup = 16;   // slots of a group
 constexpr int kPdHeads = 8;    // query heads a CTA
+constexpr int kPdMaxSplits = 256;
 constexpr float kPdLazy = 8.f;  // log2 of how far a score may pass the running maximum
 constexpr float kPdLog2e = 1.4426950408889634f;
 
@@ -48,9 +49,9 @@ struct PdRing {
   static constexpr int kRow = HD * 2;             // bytes of a row
   static constexpr int kHalf = kPdGroup * kRow;   // keys (or values) of a group
   static constexpr int kStage = 2 * kHalf;
-  // groups a warp keeps in shared memory: 96 KB (128) or 64 KB (64) a CTA, two or three CTAs an SM,
-  // 128 to 144 KB in flight on an SM
-  static constexpr int kStages = HD == 128 ? 3 : 4;
+  // groups a warp keeps in shared memory, and CTAs an SM
+  static constexpr int kStages = 3;
+  static constexpr int kCtas = HD == 128 ? 2 : 4;
   static constexpr int kBytes = kPdWarps * kStages * kStage;
   __device__ static __forceinline__ int off(int r, int ch) { return r * kRow + ((ch ^ (r & 7)) << 4); }
 };
@@ -155,7 +156,7 @@ __device__ __forceinline__ void pd_add_weights(const PdArgs &p, const PdSpan &sp
 }
 
 template <int HD, bool BF>
-__global__ void __launch_bounds__(kPdWarps * 32, HD == 128 ? 2 : 3) paged_decode_kernel(const PdArgs p) {
+__global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode_kernel(const PdArgs p) {
   using Ring = PdRing<HD>;
   constexpr int KS = HD / 16;  // k-steps of S = Q K^T
   constexpr int NT = HD / 8;   // column tiles of O
@@ -370,6 +371,7 @@ template <int HD, bool BF>
 __global__ void __launch_bounds__(kPdWarps * 32) paged_join_kernel(const PdArgs p) {
   __shared__ float2 sm_ml[128];
   __shared__ float sm_o[kPdWarps][HD];
+  __shared__ float2 sm_f[kPdMaxSplits];
   pdl_trigger();
   pdl_wait();
   const int h = blockIdx.y, i = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rep = p.a.rep;
@@ -379,20 +381,32 @@ __global__ void __launch_bounds__(kPdWarps * 32) paged_join_kernel(const PdArgs 
   if (int(blockIdx.x) < rep) {
     if (alone) return;  // the first kernel wrote it
     const int hq = h * rep + blockIdx.x;
-    const float2 tot = pd_total(p, i, hq, used, lane);
+    // every split's m and l in one round of loads, then every split's output in another
     const int64_t at = (int64_t(i) * p.a.heads + hq) * p.splits;
     constexpr int E = HD / 32;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + at;
+    const float sink = p.a.sinks ? p.a.sinks[hq] * kPdLog2e : -INFINITY;
+    for (int s = threadIdx.x; s < used; s += kPdWarps * 32) sm_f[s] = ml[s];
+    __syncthreads();
+    float m = sink;
+    for (int s = lane; s < used; s += 32) m = fmaxf(m, sm_f[s].x);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int s = lane; s < used; s += 32) l += exp2f(sm_f[s].x - ref) * sm_f[s].y;
+    l = warp_sum(l) + exp2f(sink - ref);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int s = warp; s < used; s += kPdWarps) {
-      const float f = exp2f(p.part_ml[2 * (at + s)] - tot.x);
+      const float f = exp2f(sm_f[s].x - ref);
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = fmaf(f, p.part_o[(at + s) * HD + 32 * e + lane], v[e]);
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) sm_o[warp][32 * e + lane] = v[e] * tot.y;
+    for (int e = 0; e < E; ++e) sm_o[warp][32 * e + lane] = v[e] * inv;
     __syncthreads();
     if (threadIdx.x < HD / 2) {
       const int d = 2 * threadIdx.x;
@@ -435,18 +449,22 @@ PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int max_len
     if (window == 0) return all;
     return std::min<int64_t>(all, (int64_t(first) + kPdGroup - 1) / kPdGroup + (int64_t(window) + kPdGroup - 1) / kPdGroup + 1);
   };
-  // The number of splits that makes the longest sequences' CTAs end soonest: waves of CTAs over the SMs
-  // times the rounds (a group a warp) a CTA walks, with a CTA's start and its join counted as
-  // kFixed rounds and the second kernel as as many.
-  constexpr int kFixed = 6;
-  const int64_t units = int64_t(c.seqs) * c.kv_heads * p.hgroups, slots = int64_t(sms) * (c.hd == 128 ? 2 : 3);
+  // The number of splits that ends soonest, in rounds (a group a warp) a CTA walks, its start and its join counted
+  // as kFixed rounds and the second kernel as as many. One sequence: waves of equal CTAs over the SMs. Several,
+  // whose lengths the host does not know: all of their rounds (half of what max_len allows) over the SMs, and
+  // the CTA that ends last, so that a long sequence among short ones is cut (64 sequences of up to 8,200 slots
+  // took 300 us uncut).
+  constexpr double kFixed = 6;
+  const int64_t units = int64_t(c.seqs) * c.kv_heads * p.hgroups, slots = int64_t(sms) * (c.hd == 128 ? PdRing<128>::kCtas : PdRing<64>::kCtas);
   const int64_t rounds = std::max<int64_t>(1, (groups(max_len) + kPdWarps - 1) / kPdWarps);
-  int64_t best = -1;
+  double best = -1;
   p.splits = 1;
-  for (int64_t s = 1; s <= std::min<int64_t>(rounds, 256); ++s) {
-    const int64_t per = (rounds + s - 1) / s, real = (rounds + per - 1) / per;
-    if (real != s) continue;
-    const int64_t cost = (units * s + slots - 1) / slots * (per + kFixed) + (s > 1 ? kFixed : 0);
+  for (int64_t s = 1; s <= std::min<int64_t>(rounds, kPdMaxSplits); ++s) {
+    const int64_t per = (rounds + s - 1) / s;
+    if ((rounds + per - 1) / per != s) continue;
+    double cost = s > 1 ? kFixed : 0;
+    if (c.seqs == 1) cost += double((units * s + slots - 1) / slots) * (per + kFixed);
+    else cost += 0.5 * units * (s * kFixed + rounds) / slots + per + kFixed;
     if (best < 0 || cost < best) {
       best = cost;
       p.splits = int(s);

@@ -47,15 +47,20 @@ class PagedCache:
                                      k.stride(2), block_table.stride(0), _TYPES[str(k.dtype)], seqs, heads, dim, page,
                                      pages, width, 0)
         self._ref = C.addressof(self.desc)
+        self._int32 = block_table.dtype
 
     def _attn(self, q, out, scale, window, first, sinks):
         rows, heads, dim = q.shape
-        _need(q.dtype == self.dtype and out.dtype == self.dtype, "PagedCache: q and out must have the cache's type")
-        _need(out.shape == q.shape and dim == self.head_dim, "PagedCache: q and out must be [rows][heads][head_dim]")
+        dtype = self.dtype
+        if q.dtype != dtype or out.dtype != dtype:
+            raise A.HcError("PagedCache: q and out must have the cache's type")
+        if out.shape != q.shape or dim != self.head_dim:
+            raise A.HcError("PagedCache: q and out must be [rows][heads][head_dim]")
         qs, os = q.stride(), out.stride()
-        _need(qs[2] == 1 and os[2] == 1, "PagedCache: the last dimension of q and out must be contiguous")
+        if qs[2] != 1 or os[2] != 1:
+            raise A.HcError("PagedCache: the last dimension of q and out must be contiguous")
         if sinks is not None:
-            _need(str(sinks.dtype).endswith("float32") and tuple(sinks.shape) == (heads,) and sinks.is_contiguous(),
+            _need(str(sinks.dtype).endswith("float32") and sinks.shape == (heads,) and sinks.is_contiguous(),
                   "PagedCache: sinks must be float32 [heads]")
             sinks = sinks.data_ptr()
         return A.PagedAttn(q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], sinks, scale, heads, window, first)
@@ -65,20 +70,22 @@ class PagedCache:
         if scratch is None:
             return None, 0
         _need(scratch.is_contiguous(), "PagedCache: scratch must be contiguous")
-        return scratch.data_ptr(), scratch.numel() * scratch.element_size()
+        return scratch.data_ptr(), scratch.nbytes
 
     def append(self, k, v, seq, slot, stream=None):
         """Writes rows k, v [rows][kv_heads][head_dim] into slot[r] of sequence seq[r] (int32 [rows]);
         a negative slot leaves its row out. Lengths are the caller's to move."""
         rows = k.shape[0]
-        _need(k.dtype == self.dtype and v.dtype == self.dtype, "PagedCache.append: k and v must have the cache's type")
-        _need(tuple(k.shape) == (rows, self.kv_heads, self.head_dim) and tuple(v.shape) == tuple(k.shape),
-              "PagedCache.append: k and v must be [rows][kv_heads][head_dim]")
+        if k.dtype != self.dtype or v.dtype != self.dtype:
+            raise A.HcError("PagedCache.append: k and v must have the cache's type")
+        if k.shape != (rows, self.kv_heads, self.head_dim) or v.shape != k.shape:
+            raise A.HcError("PagedCache.append: k and v must be [rows][kv_heads][head_dim]")
         ks, vs = k.stride(), v.stride()
-        _need(ks[2] == 1 and vs[2] == 1, "PagedCache.append: the last dimension of k and v must be contiguous")
+        if ks[2] != 1 or vs[2] != 1:
+            raise A.HcError("PagedCache.append: the last dimension of k and v must be contiguous")
         for t in (seq, slot):
-            _need(str(t.dtype).endswith("int32") and tuple(t.shape) == (rows,) and t.is_contiguous(),
-                  "PagedCache.append: seq and slot must be int32 [rows]")
+            if t.dtype != self._int32 or t.shape != (rows,) or not t.is_contiguous():
+                raise A.HcError("PagedCache.append: seq and slot must be int32 [rows]")
         A.check(A.lib().hc_paged_append_run(self._ref, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
                                             seq.data_ptr(), slot.data_ptr(), rows, stream))
 
@@ -106,8 +113,8 @@ class PagedCache:
         starts[i] .. starts[i + 1] - 1 of q, out [rows][heads][head_dim] are sequence i's last slots
         (starts int32 [seqs + 1]; no sequence has more than max_rows of them)."""
         _need(len(q.shape) == 3, "PagedCache.prompt: q must be [rows][heads][head_dim]")
-        _need(str(starts.dtype).endswith("int32") and tuple(starts.shape) == (self.seqs + 1,) and starts.is_contiguous(),
-              "PagedCache.prompt: starts must be int32 [seqs + 1]")
+        if starts.dtype != self._int32 or starts.shape != (self.seqs + 1,) or not starts.is_contiguous():
+            raise A.HcError("PagedCache.prompt: starts must be int32 [seqs + 1]")
         a = self._attn(q, out, scale, window, first, sinks)
         p, n = self._scratch(scratch)
         A.check(A.lib().hc_paged_prompt_run(self._ref, C.addressof(a), starts.data_ptr(), q.shape[0], max_rows, max_len,
@@ -125,8 +132,8 @@ class PagedCache:
         kept (int32 [seqs][kv_heads][keep], the slots they came from, -1 past the new length)."""
         _need(isinstance(to, PagedCache), "PagedCache.evict: `to` must be a PagedCache")
         if kept is not None:
-            _need(str(kept.dtype).endswith("int32") and tuple(kept.shape) == (self.seqs, self.kv_heads, keep)
-                  and kept.is_contiguous(), "PagedCache.evict: kept must be int32 [seqs][kv_heads][keep]")
+            _need(kept.dtype == self._int32 and kept.shape == (self.seqs, self.kv_heads, keep) and kept.is_contiguous(),
+                  "PagedCache.evict: kept must be int32 [seqs][kv_heads][keep]")
         p, n = self._scratch(scratch)
         A.check(A.lib().hc_paged_evict_run(self._ref, to._ref, keep, first, recent, max_len,
                                            kept.data_ptr() if kept is not None else None, p, n, stream))
