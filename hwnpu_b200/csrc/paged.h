@@ -53,6 +53,11 @@ cudaError_t paged_evict(const PagedView &c, const PagedView &to, int keep, int f
 size_t paged_decode_scratch(const PagedView &c, int heads, int window, int first, int max_len, bool accumulate, int sms);
 cudaError_t paged_decode(const PagedView &c, const PagedQuery &a, int max_len, bool accumulate, void *scratch, int sms,
                          cudaStream_t st);
+// Whether a prompt call is one of few rows (tokens times query heads a kv head), which run as decode does.
+bool paged_few(const PagedView &c, int heads, int max_rows);
+size_t paged_few_scratch(const PagedView &c, int heads, int window, int first, int rows, int max_len, int sms);
+cudaError_t paged_few_run(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows, int max_rows,
+                          int max_len, void *scratch, int sms, cudaStream_t st);
 size_t paged_prompt_scratch(const PagedView &c, int heads, int window, int first, int rows, int max_rows, int max_len,
                             int sms);
 cudaError_t paged_prompt(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows, int max_rows,

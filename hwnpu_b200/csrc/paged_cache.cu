@@ -44,37 +44,22 @@ constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048;
 constexpr int kSelCache = 49152;  // keys a CTA can hold in shared memory (192 KB)
 
-// Exclusive prefix sum over the CTA's threads of two counts in one word each; *total: the sums.
-__device__ __forceinline__ longlong2 sel_scan(long long a, long long b, longlong2 *warps, longlong2 *total) {
+// Exclusive prefix sum of v over the CTA's threads.
+__device__ __forceinline__ int sel_scan(int v, int *warps) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = a, y = b;
+  int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
-    if (lane >= o) {
-      x += u;
-      y += v;
-    }
+    const int u = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += u;
   }
-  if (lane == 31) warps[warp] = make_longlong2(x, y);
+  if (lane == 31) warps[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    const longlong2 w = warps[lane];
-    long long p = w.x, q = w.y;
+  int before = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, p, o), v = __shfl_up_sync(0xffffffffu, q, o);
-      if (lane >= o) {
-        p += u;
-        q += v;
-      }
-    }
-    warps[lane] = make_longlong2(p - w.x, q - w.y);
-    if (lane == 31) *total = make_longlong2(p, q);
-  }
+  for (int w = 0; w < kSelThreads / 32; ++w) before += w < warp ? warps[w] : 0;
   __syncthreads();
-  const longlong2 before = warps[warp];
-  return make_longlong2(before.x + x - a, before.y + y - b);
+  return before + x - v;
 }
 
 // One CTA a (sequence, kv head): the slots to keep into idx, ascending. The key of the last candidate that stays
@@ -82,17 +67,19 @@ __device__ __forceinline__ longlong2 sel_scan(long long a, long long b, longlong
 // memory (a row of up to 49,152; longer ones are read again, from the L2 cache); then every thread counts what
 // stays of a run of candidates, and writes it behind what the threads before it count.
 //
-// Bound by the passes over a row by one SM, not by its bytes (128 rows of up to 32,771 weights: 14 MB).
+// Bound by the passes over a row by one SM, not by its bytes: 128 rows of up to 32,771 weights (10 MB) take 40 us, one
+// CTA an SM. Adding a warp's equal digits at once (ballots), or loading 4 or 8 keys ahead, was no faster, and rows of
+// one value are not slower without.
 __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, int keep, int first, int recent, int cache,
                                                                    int32_t *__restrict__ idx,
                                                                    int32_t *__restrict__ to_lengths) {
   extern __shared__ uint32_t sel_keys[];
   __shared__ int hist[kSelBins];
-  __shared__ longlong2 warps[32], total;
+  __shared__ int warps[kSelThreads / 32];
   __shared__ int sh_digit, sh_above;
   pdl_trigger();
   pdl_wait();
-  const int h = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int h = blockIdx.x, i = blockIdx.y, tid = threadIdx.x;
   const int n = paged_len(c, i);
   int32_t *out = idx + (int64_t(i) * c.kv_heads + h) * keep;
   if (h == 0 && tid == 0) to_lengths[i] = min(n, keep);
@@ -116,36 +103,22 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
     for (int j0 = 0; j0 < cand; j0 += kSelThreads) {
       const int j = j0 + tid;
       uint32_t key = 0;
-      bool in = j < cand;
-      if (in) {
-        if (pass == 0 || !cached) {
-          key = weight_key(w[j]);
-          if (cached) sel_keys[j] = key;
-        } else {
-          key = sel_keys[j];
-        }
-        in = (key & known) == prefix;
+      if (j < cand) {
+        key = pass == 0 || !cached ? weight_key(w[j]) : sel_keys[j];
+        if (pass == 0 && cached) sel_keys[j] = key;
       }
+      const bool in = j < cand && (key & known) == prefix;
       const int digit = (key >> shift) & ((1 << bits) - 1);
-      // a warp whose keys all have one digit (rows of zeros) adds once instead of in 32 turns
-      const unsigned who = __ballot_sync(0xffffffffu, in);
-      if (who) {
-        const int lead = __shfl_sync(0xffffffffu, digit, __ffs(who) - 1);
-        if (__all_sync(0xffffffffu, !in || digit == lead)) {
-          if (lane == 0) atomicAdd(&hist[lead], __popc(who));
-        } else if (in) {
-          atomicAdd(&hist[digit], 1);
-        }
-      }
+      if (in) atomicAdd(&hist[digit], 1);
     }
     __syncthreads();
     // thread t holds bins 2 t and 2 t + 1 from the largest digit down
     const int d0 = kSelBins - 1 - 2 * tid, n0 = hist[d0], n1 = hist[d0 - 1];
-    const longlong2 above = sel_scan(n0 + n1, 0, warps, &total);
-    if (above.x < need && above.x + n0 + n1 >= need) {
-      const bool upper = above.x + n0 >= need;
+    const int above = sel_scan(n0 + n1, warps);
+    if (above < need && above + n0 + n1 >= need) {
+      const bool upper = above + n0 >= need;
       sh_digit = upper ? d0 : d0 - 1;
-      sh_above = int(above.x) + (upper ? 0 : n0);
+      sh_above = above + (upper ? 0 : n0);
     }
     __syncthreads();
     prefix |= uint32_t(sh_digit) << shift;
@@ -162,8 +135,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
     gt += key > prefix;
     eq += key == prefix;
   }
-  const longlong2 before = sel_scan(gt, eq, warps, &total);
-  int ties = int(min((long long)need, before.y)), at = first + int(before.x) + ties;
+  const int over = sel_scan(gt, warps);
+  int ties = min(need, sel_scan(eq, warps)), at = first + over + ties;
   for (int j = j0; j < j1; ++j) {
     const uint32_t key = cached ? sel_keys[j] : weight_key(w[j]);
     const bool tie = key == prefix && ties < need;
@@ -175,8 +148,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
 }
 
 // Copies the kept rows: a thread has a 16-byte piece of kCopyRows rows, keys and values, all loaded before the
-// first is stored. Bound by HBM (540 MB in 90 us at 4,096 of up to 32,771 rows for 16 sequences of 8
-// heads: 6.0 TB/s).
+// first is stored. Bound by HBM: 4,096 rows a head of 16 sequences of 8 heads of 128, 270 MB read and as much
+// written, take 93 us (5.3 TB/s).
 constexpr int kCopyRows = 4;
 template <int CH>
 __global__ void __launch_bounds__(256) paged_copy_kernel(PagedView c, PagedView to, int keep,

@@ -1,6 +1,7 @@
 // paged_decode.cu: attention of one new token a sequence over a caller's paged 16-bit cache
-// (hc_paged_decode_run): softmax(scale q K^T) V over the visible slots, the cache's length split over
-// CTAs and joined (Flash-Decoding, paged.go:227-310).
+// (hc_paged_decode_run), and of a few (hc_paged_prompt_run with up to 16 rows of tokens times query heads
+// a kv head: a speculative verify): softmax(scale q K^T) V over the visible slots, the cache's
+// length split over CTAs and joined (Flash-Decoding, paged.go:227-310).
 //
 // Bound. A visible slot costs 4 head_dim bytes of HBM (its key and its value, once for all the query
 // heads of the kv head) and 4 head_dim flops a query head: at most 8 flops a byte with 8 heads, far
@@ -23,6 +24,7 @@
 //   O += P V     the same MMA: rows 0-7 of A are P rounded to the cache's type, rows 8-15 what the
 //                rounding left of P (rounded in its turn), so that the weights carry 16 bits or more
 //                at no further MMA; B is V by ldmatrix.trans. O is float32
+// Of several tokens both halves of A are rows, and the weights are rounded to the cache's type once.
 // The four warps' (m, l, O) are joined in shared memory, the splits' by a second kernel, both in a
 // fixed order. With `accumulate` the scores are kept in scratch (float32) and the visible slots' weights
 // exp2(S - m) / l are summed over the heads once m and l are known.
@@ -41,6 +43,7 @@ constexpr int kPdWarps = 4;
 constexpr int kPdGroup = 16;   // slots of a group
 constexpr int kPdHeads = 8;    // query heads a CTA
 constexpr int kPdMaxSplits = 256;
+constexpr int kPdFew = 16;     // rows of several tokens a CTA
 constexpr float kPdLazy = 8.f;  // log2 of how far a score may pass the running maximum
 constexpr float kPdLog2e = 1.4426950408889634f;
 
@@ -111,12 +114,12 @@ __device__ __forceinline__ float2 pd_unpack(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
-// The visible slots of a query at slot n - 1 as groups of 16: ga of them from slot 0 on, then gb from slot
-// 16 b0 on; slot j of them is seen when j < n and (j >= lo or j < first).
+// The slots that queries at slots qmin .. n - 1 see, as groups of 16: ga of them from slot 0 on, then those from
+// slot 16 b0 on; slot j of them is seen by one of the queries when j < n and (j >= lo or j < first).
 struct PdSpan {
   int n, lo, first, ga, b0, groups;
-  __device__ __forceinline__ PdSpan(int len, int window, int first_) : n(len), first(first_) {
-    lo = window > 0 && n > window ? n - window : 0;
+  __device__ __forceinline__ PdSpan(int n_, int qmin, int window, int first_) : n(n_) {
+    lo = window > 0 && qmin >= window ? qmin - window + 1 : 0;
     first = min(first_, lo);
     ga = (first + kPdGroup - 1) / kPdGroup;
     b0 = max(lo / kPdGroup, ga);
@@ -136,9 +139,30 @@ struct PdArgs {
   int splits, hgroups;
   bool accumulate;
   int64_t score_stride;  // scores a head keeps in scratch
-  float *part_ml;        // [seqs][heads][splits][2]: m (log2 units) and l
-  float *part_o;         // [seqs][heads][splits][hd], not divided by l
+  float *part_ml;        // [rows][heads][splits][2]: m (log2 units) and l
+  float *part_o;         // [rows][heads][splits][hd], not divided by l
   float *scores;         // [seqs][heads][score_stride], log2 units, by group
+  const int32_t *starts; // of hc_paged_prompt_run, or null: one row a sequence
+  int rows, max_rows;
+};
+
+// The rows of sequence i: q rows row0 .. row0 + count - 1, the token t at slot p0 + t.
+struct PdRows {
+  int row0, count, p0;
+  __device__ __forceinline__ PdRows(const PdArgs &p, int i) {
+    const int len = paged_len(p.c, i);
+    row0 = i;
+    count = 1;
+    p0 = len - 1;
+    if (p.starts) {
+      row0 = p.starts[i];
+      const int cnt = p.starts[i + 1] - row0;
+      const bool there = row0 >= 0 && row0 <= p.rows && cnt > 0;
+      count = there ? min(min(cnt, p.max_rows), p.rows - row0) : 0;
+      p0 = len - cnt;
+    }
+  }
+  __device__ __forceinline__ PdSpan span(const PdArgs &p) const { return PdSpan(max(0, p0 + count), p0, p.a.window, p.a.first); }
 };
 
 // The weights of groups [g0, g1) of (sequence i, kv head h), once each head's m and 1 / l are in ml.
@@ -155,30 +179,38 @@ __device__ __forceinline__ void pd_add_weights(const PdArgs &p, const PdSpan &sp
   }
 }
 
-template <int HD, bool BF>
+// MANY: up to 16 rows, the tokens of a sequence times the query heads of a kv head (row = token * rep + head),
+// in both halves of A; else the query heads of one token, at most 8.
+template <int HD, bool BF, bool MANY>
 __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode_kernel(const PdArgs p) {
   using Ring = PdRing<HD>;
   constexpr int KS = HD / 16;  // k-steps of S = Q K^T
   constexpr int NT = HD / 8;   // column tiles of O
   constexpr int CH = HD / 8;   // 16-byte pieces of a row
   constexpr int RPS = 32 / CH;  // rows a warp copies an instruction
+  constexpr int HALVES = MANY ? 2 : 1, ROWS = 8 * HALVES;
   // P is held 2^kBias above exp2(S - m): fp16's smallest weights, 2^-25, then stand for 2^-32, and its
   // largest for 2^15
   constexpr float kBias = BF ? 0.f : 7.f;
   extern __shared__ __align__(128) uint8_t pd_buf[];
-  __shared__ float sm_m[kPdWarps][kPdHeads], sm_l[kPdWarps][kPdHeads];
-  __shared__ float2 sm_ml[kPdHeads];
+  __shared__ float sm_m[kPdWarps][ROWS], sm_l[kPdWarps][ROWS];
+  __shared__ float2 sm_ml[ROWS];
   pdl_trigger();
   pdl_wait();
   const PagedView &c = p.c;
   const int split = blockIdx.x, h = blockIdx.y / p.hgroups, hg = blockIdx.y % p.hgroups, i = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, cq = lane & 3;
-  const PdSpan sp(paged_len(c, i), p.a.window, p.a.first);
+  const PdRows rw(p, i);
+  if (rw.count <= 0) return;
+  const PdSpan sp = rw.span(p);
   const int per = sp.per(p.splits);
   const int g0 = split * per, g1 = min(sp.groups, g0 + per);
   if (g0 >= g1 && split > 0) return;
   const bool alone = sp.groups <= per;  // this CTA has the whole row
-  const int head0 = h * p.a.rep + hg * kPdHeads, nheads = min(kPdHeads, p.a.rep - hg * kPdHeads);
+  const int rep = p.a.rep, head0 = h * rep + hg * kPdHeads;
+  const int nrows = MANY ? rw.count * rep : min(kPdHeads, rep - hg * kPdHeads);
+  // groups that every row sees: below the first one's slot, from the last one's window on
+  const int qmin = rw.p0, lo_all = p.a.window > 0 ? rw.p0 + rw.count - p.a.window : 0;
 
   // the warp's page ids: lane k has that of its k-th group from `at` on, the next 32 are on their way
   const int32_t *table = c.table + i * c.table_stride;
@@ -220,22 +252,33 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
 #pragma unroll
   for (int k = 0; k < Ring::kStages - 1; ++k) issue(k);
 
-  // the query heads as A fragments (rows 8-15 are zero)
-  uint32_t qa[KS][2];
-  {
-    const uint16_t *q = p.a.q + i * p.a.q_row + (head0 + gq) * p.a.q_head + 2 * cq;
+  // the rows as A fragments (rows 8-15 are zero for a single token)
+  uint32_t qa[KS][2][HALVES];
+  int pos[HALVES];  // the rows' slots
+#pragma unroll
+  for (int b = 0; b < HALVES; ++b) {
+    const int r = gq + 8 * b, tok = MANY ? r / rep : 0;
+    const bool there = r < nrows;
+    const uint16_t *q = p.a.q + int64_t(rw.row0 + tok) * p.a.q_row + (head0 + r - tok * rep) * p.a.q_head + 2 * cq;
+    pos[b] = there ? rw.p0 + tok : -1;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      qa[s][0] = gq < nheads ? *reinterpret_cast<const uint32_t *>(q + 16 * s) : 0u;
-      qa[s][1] = gq < nheads ? *reinterpret_cast<const uint32_t *>(q + 16 * s + 8) : 0u;
+      qa[s][0][b] = there ? *reinterpret_cast<const uint32_t *>(q + 16 * s) : 0u;
+      qa[s][1][b] = there ? *reinterpret_cast<const uint32_t *>(q + 16 * s + 8) : 0u;
     }
   }
   const float scale2 = p.a.scale * kPdLog2e;  // scores in log2 units
-  float m = -INFINITY, l = 0.f;                          // of head gq, the same on its 4 lanes (l: this lane's part)
+  float m[HALVES], l[HALVES];  // of row gq (and gq + 8), the same on its 4 lanes (l: this lane's part)
+#pragma unroll
+  for (int b = 0; b < HALVES; ++b) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+  }
   float o[NT][4];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-  float *score_row = p.accumulate && gq < nheads ? p.scores + (int64_t(i) * p.a.heads + head0 + gq) * p.score_stride : nullptr;
+  float *score_row =
+      !MANY && p.accumulate && gq < nrows ? p.scores + (int64_t(i) * p.a.heads + head0 + gq) * p.score_stride : nullptr;
   const int lm = lane >> 3, lr = lane & 7;
 
   for (int k = 0; g0 + warp + k * kPdWarps < g1; ++k) {
@@ -249,74 +292,105 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
     for (int s = 0; s < KS; ++s) {
       uint32_t b[4];
       pd_ldsm4<false>(buf + Ring::off((lm >> 1) * 8 + lr, 2 * s + (lm & 1)), b);
-      pd_mma<BF>(s0, qa[s][0], 0u, qa[s][1], 0u, b[0], b[1]);
-      pd_mma<BF>(s1, qa[s][0], 0u, qa[s][1], 0u, b[2], b[3]);
+      const uint32_t q1 = MANY ? qa[s][0][HALVES - 1] : 0u, q3 = MANY ? qa[s][1][HALVES - 1] : 0u;
+      pd_mma<BF>(s0, qa[s][0][0], q1, qa[s][1][0], q3, b[0], b[1]);
+      pd_mma<BF>(s1, qa[s][0][0], q1, qa[s][1][0], q3, b[2], b[3]);
     }
     const int j0 = sp.slot(g);
-    float x[4] = {s0[0] * scale2, s0[1] * scale2, s1[0] * scale2, s1[1] * scale2};  // slots 2c, 2c+1, 8+2c, 9+2c
-    if (!(j0 + kPdGroup <= sp.n && (j0 >= sp.lo || j0 + kPdGroup <= sp.first))) {
+    const bool whole = j0 + kPdGroup - 1 <= qmin && (j0 >= lo_all || j0 + kPdGroup <= p.a.first);
+    float x[HALVES][4];  // slots 2c, 2c+1, 8+2c, 9+2c
+    bool move = false;
+    float mx[HALVES];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (!sp.sees(j0 + 2 * cq + (e & 1) + 8 * (e >> 1))) x[e] = -INFINITY;
+    for (int b = 0; b < HALVES; ++b) {
+      x[b][0] = s0[2 * b] * scale2;
+      x[b][1] = s0[2 * b + 1] * scale2;
+      x[b][2] = s1[2 * b] * scale2;
+      x[b][3] = s1[2 * b + 1] * scale2;
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + 2 * cq + (e & 1) + 8 * (e >> 1);
+          if (!(j <= pos[b] && (p.a.window == 0 || pos[b] - j < p.a.window || j < p.a.first))) x[b][e] = -INFINITY;
+        }
+      }
+      mx[b] = fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3]));
+      mx[b] = fmaxf(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 1));
+      mx[b] = fmaxf(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 2));
+      move = move || mx[b] > m[b] + kPdLazy;
     }
     if (score_row) {
-      *reinterpret_cast<float2 *>(score_row + g * kPdGroup + 2 * cq) = make_float2(x[0], x[1]);
-      *reinterpret_cast<float2 *>(score_row + g * kPdGroup + 8 + 2 * cq) = make_float2(x[2], x[3]);
+      *reinterpret_cast<float2 *>(score_row + g * kPdGroup + 2 * cq) = make_float2(x[0][0], x[0][1]);
+      *reinterpret_cast<float2 *>(score_row + g * kPdGroup + 8 + 2 * cq) = make_float2(x[0][2], x[0][3]);
     }
-    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    if (__any_sync(0xffffffffu, mx > m + kPdLazy || (m == -INFINITY && mx > m))) {
-      const float nm = fmaxf(m, mx);
-      const float f = m == -INFINITY ? 0.f : exp2f(m - nm);
-      m = nm;
-      l *= f;
+    if (__any_sync(0xffffffffu, move)) {
+      float f[2];
+#pragma unroll
+      for (int b = 0; b < HALVES; ++b) {
+        const float nm = fmaxf(m[b], mx[b]);
+        f[b] = m[b] == -INFINITY ? 0.f : exp2f(m[b] - nm);
+        m[b] = nm;
+        l[b] *= f[b];
+      }
+      if (!MANY) f[1] = f[0];  // what rounding left of rows 0-7 belongs to the same heads
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        // rows 0-7 and what their rounding left, rows 8-15, belong to one head
-        o[t][0] *= f;
-        o[t][1] *= f;
-        o[t][2] *= f;
-        o[t][3] *= f;
+        o[t][0] *= f[0];
+        o[t][1] *= f[0];
+        o[t][2] *= f[1];
+        o[t][3] *= f[1];
       }
     }
-    const float ref = m == -INFINITY ? 0.f : m - kBias;
-    float e[4];
+    uint32_t pa[4];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      e[y] = exp2f(x[y] - ref);
-      l += e[y];
+    for (int b = 0; b < HALVES; ++b) {
+      const float ref = m[b] == -INFINITY ? 0.f : m[b] - kBias;
+      float e[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        e[y] = exp2f(x[b][y] - ref);
+        l[b] += e[y];
+      }
+      pa[b] = pd_pack<BF>(e[0], e[1]);
+      pa[2 + b] = pd_pack<BF>(e[2], e[3]);
+      if (!MANY) {
+        const float2 h0 = pd_unpack<BF>(pa[0]), h1 = pd_unpack<BF>(pa[2]);
+        pa[1] = pd_pack<BF>(e[0] - h0.x, e[1] - h0.y);
+        pa[3] = pd_pack<BF>(e[2] - h1.x, e[3] - h1.y);
+      }
     }
-    const uint32_t p0 = pd_pack<BF>(e[0], e[1]), p1 = pd_pack<BF>(e[2], e[3]);
-    const float2 h0 = pd_unpack<BF>(p0), h1 = pd_unpack<BF>(p1);
-    const uint32_t r0 = pd_pack<BF>(e[0] - h0.x, e[1] - h0.y), r1 = pd_pack<BF>(e[2] - h1.x, e[3] - h1.y);
 #pragma unroll
     for (int t = 0; t < NT; t += 2) {
       uint32_t b[4];
       pd_ldsm4<true>(buf + Ring::kHalf + Ring::off((lm & 1) * 8 + lr, t + (lm >> 1)), b);
-      pd_mma<BF>(o[t], p0, r0, p1, r1, b[0], b[1]);
-      pd_mma<BF>(o[t + 1], p0, r0, p1, r1, b[2], b[3]);
+      pd_mma<BF>(o[t], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+      pd_mma<BF>(o[t + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
     }
     __syncwarp();  // the stage is read before it is filled again
   }
   pd_wait<0>();
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
   __syncthreads();  // every warp is done with its ring
 
-  // join the warps: [warp][head][hd] float32 in the ring's memory
+  // join the warps: [warp][row][hd] float32 in the ring's memory
   float *po = reinterpret_cast<float *>(pd_buf);
-  if (cq == 0) {
-    sm_m[warp][gq] = m - kBias;
-    sm_l[warp][gq] = l;
-  }
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-    *reinterpret_cast<float2 *>(po + (warp * kPdHeads + gq) * HD + 8 * t + 2 * cq) =
-        make_float2(o[t][0] + o[t][2], o[t][1] + o[t][3]);
+  for (int b = 0; b < HALVES; ++b) {
+    l[b] += __shfl_xor_sync(0xffffffffu, l[b], 1);
+    l[b] += __shfl_xor_sync(0xffffffffu, l[b], 2);
+    if (cq == 0) {
+      sm_m[warp][gq + 8 * b] = m[b] - kBias;
+      sm_l[warp][gq + 8 * b] = l[b];
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float2 v = MANY ? make_float2(o[t][2 * b], o[t][2 * b + 1]) : make_float2(o[t][0] + o[t][2], o[t][1] + o[t][3]);
+      *reinterpret_cast<float2 *>(po + (warp * ROWS + gq + 8 * b) * HD + 8 * t + 2 * cq) = v;
+    }
+  }
   __syncthreads();
-  for (int u = threadIdx.x; u < nheads * (HD / 2); u += kPdWarps * 32) {
-    const int r = u / (HD / 2), d = 2 * (u % (HD / 2)), hq = head0 + r;
+  for (int u = threadIdx.x; u < nrows * (HD / 2); u += kPdWarps * 32) {
+    const int r = u / (HD / 2), d = 2 * (u % (HD / 2)), tok = MANY ? r / rep : 0;
+    const int hq = head0 + r - tok * rep, row = rw.row0 + tok;
     float mm = sm_m[0][r];
 #pragma unroll
     for (int w = 1; w < kPdWarps; ++w) mm = fmaxf(mm, sm_m[w][r]);
@@ -326,7 +400,7 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
 #pragma unroll
     for (int w = 0; w < kPdWarps; ++w) {
       const float f = exp2f(sm_m[w][r] - ref);
-      const float2 v = *reinterpret_cast<const float2 *>(po + (w * kPdHeads + r) * HD + d);
+      const float2 v = *reinterpret_cast<const float2 *>(po + (w * ROWS + r) * HD + d);
       ll += f * sm_l[w][r];
       vx += f * v.x;
       vy += f * v.y;
@@ -334,18 +408,18 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
     if (alone) {
       // the heads of one kv head are spread over CTAs: the second kernel adds the weights
       if (p.accumulate && p.hgroups > 1 && d == 0)
-        *reinterpret_cast<float2 *>(p.part_ml + 2 * (int64_t(i) * p.a.heads + hq) * p.splits) = make_float2(mm, ll);
+        *reinterpret_cast<float2 *>(p.part_ml + 2 * (int64_t(row) * p.a.heads + hq) * p.splits) = make_float2(mm, ll);
       if (p.a.sinks) ll += exp2f(p.a.sinks[hq] * kPdLog2e - ref);
       const float inv = ll > 0.f ? 1.f / ll : 0.f;
-      *reinterpret_cast<uint32_t *>(p.a.o + i * p.a.o_row + hq * p.a.o_head + d) = pd_pack<BF>(vx * inv, vy * inv);
+      *reinterpret_cast<uint32_t *>(p.a.o + row * p.a.o_row + hq * p.a.o_head + d) = pd_pack<BF>(vx * inv, vy * inv);
       if (d == 0) sm_ml[r] = make_float2(ref, inv);
     } else {
-      const int64_t at = (int64_t(i) * p.a.heads + hq) * p.splits + split;
+      const int64_t at = (int64_t(row) * p.a.heads + hq) * p.splits + split;
       *reinterpret_cast<float2 *>(p.part_o + at * HD + d) = make_float2(vx, vy);
       if (d == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(mm, ll);
     }
   }
-  if (p.accumulate && alone && p.hgroups == 1) {
+  if (!MANY && p.accumulate && alone && p.hgroups == 1) {
     __syncthreads();
     pd_add_weights(p, sp, i, h, 0, sp.groups, sm_ml);
   }
@@ -365,24 +439,26 @@ __device__ __forceinline__ float2 pd_total(const PdArgs &p, int i, int hq, int u
   return make_float2(m, 1.f / l);
 }
 
-// Joins the splits of (sequence, kv head): CTAs x < rep the output of query head x, 4 warps taking
-// every fourth split; the others the weights, a share of the groups each.
+// Joins the splits of (sequence, kv head): CTAs x < outs (query heads, times tokens) the output of row x, 4 warps
+// taking every fourth split; the others the weights, a share of the groups each.
 template <int HD, bool BF>
-__global__ void __launch_bounds__(kPdWarps * 32) paged_join_kernel(const PdArgs p) {
+__global__ void __launch_bounds__(kPdWarps * 32) paged_join_kernel(const PdArgs p, int outs) {
   __shared__ float2 sm_ml[128];
   __shared__ float sm_o[kPdWarps][HD];
   __shared__ float2 sm_f[kPdMaxSplits];
   pdl_trigger();
   pdl_wait();
   const int h = blockIdx.y, i = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rep = p.a.rep;
-  const PdSpan sp(paged_len(p.c, i), p.a.window, p.a.first);
+  const PdRows rw(p, i);
+  if (rw.count <= 0) return;
+  const PdSpan sp = rw.span(p);
   const int per = sp.per(p.splits), used = max(1, (sp.groups + per - 1) / per);
   const bool alone = used == 1;
-  if (int(blockIdx.x) < rep) {
-    if (alone) return;  // the first kernel wrote it
-    const int hq = h * rep + blockIdx.x;
+  if (int(blockIdx.x) < outs) {
+    const int tok = blockIdx.x / rep, hq = h * rep + blockIdx.x % rep, row = rw.row0 + tok;
+    if (alone || tok >= rw.count) return;  // the first kernel wrote it
     // every split's m and l in one round of loads, then every split's output in another
-    const int64_t at = (int64_t(i) * p.a.heads + hq) * p.splits;
+    const int64_t at = (int64_t(row) * p.a.heads + hq) * p.splits;
     constexpr int E = HD / 32;
     const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + at;
     const float sink = p.a.sinks ? p.a.sinks[hq] * kPdLog2e : -INFINITY;
@@ -416,12 +492,12 @@ __global__ void __launch_bounds__(kPdWarps * 32) paged_join_kernel(const PdArgs 
         x += sm_o[w][d];
         y += sm_o[w][d + 1];
       }
-      *reinterpret_cast<uint32_t *>(p.a.o + i * p.a.o_row + hq * p.a.o_head + d) = pd_pack<BF>(x, y);
+      *reinterpret_cast<uint32_t *>(p.a.o + row * p.a.o_row + hq * p.a.o_head + d) = pd_pack<BF>(x, y);
     }
     return;
   }
   if (alone && p.hgroups == 1) return;  // the first kernel added them
-  const int wb = gridDim.x - rep, share = (sp.groups + wb - 1) / wb, g0 = (int(blockIdx.x) - rep) * share;
+  const int wb = gridDim.x - outs, share = (sp.groups + wb - 1) / wb, g0 = (int(blockIdx.x) - outs) * share;
   if (g0 >= sp.groups) return;
   for (int r = warp; r < rep; r += kPdWarps) {
     const float2 tot = pd_total(p, i, h * rep + r, used, lane);
@@ -441,18 +517,20 @@ struct PdPlan {
 
 size_t pd_up(size_t n) { return (n + 255) / 256 * 256; }
 
-PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int max_len, bool accumulate, int sms) {
+// rows: q rows in all; few: of several a sequence (MANY).
+PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int rows, bool few, int max_len, bool accumulate,
+               int sms) {
   PdPlan p{};
-  p.hgroups = (heads / c.kv_heads + kPdHeads - 1) / kPdHeads;
+  p.hgroups = few ? 1 : (heads / c.kv_heads + kPdHeads - 1) / kPdHeads;
   auto groups = [&](int len) -> int64_t {
     const int64_t all = (int64_t(len) + kPdGroup - 1) / kPdGroup;
     if (window == 0) return all;
-    return std::min<int64_t>(all, (int64_t(first) + kPdGroup - 1) / kPdGroup + (int64_t(window) + kPdGroup - 1) / kPdGroup + 1);
+    return std::min<int64_t>(all, (int64_t(first) + kPdGroup - 1) / kPdGroup + (int64_t(window) + (few ? kPdFew : 0) + kPdGroup - 1) / kPdGroup + 1);
   };
   // The number of splits that ends soonest, in rounds (a group a warp) a CTA walks, its start and its join counted
   // as kFixed rounds and the second kernel as as many. One sequence: waves of equal CTAs over the SMs. Several,
-  // whose lengths the host does not know: all of their rounds (half of what max_len allows) over the SMs, and
-  // the CTA that ends last, so that a long sequence among short ones is cut (64 sequences of up to 8,200 slots
+  // whose lengths the host does not know: where not all CTAs fit at once, all rounds (half of what max_len allows)
+  // over the SMs, and then the CTA that ends last, so that a long sequence among short ones is cut (64 sequences of up to 8,200 slots
   // took 300 us uncut).
   constexpr double kFixed = 6;
   const int64_t units = int64_t(c.seqs) * c.kv_heads * p.hgroups, slots = int64_t(sms) * (c.hd == 128 ? PdRing<128>::kCtas : PdRing<64>::kCtas);
@@ -464,7 +542,7 @@ PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int max_len
     if ((rounds + per - 1) / per != s) continue;
     double cost = s > 1 ? kFixed : 0;
     if (c.seqs == 1) cost += double((units * s + slots - 1) / slots) * (per + kFixed);
-    else cost += 0.5 * units * (s * kFixed + rounds) / slots + per + kFixed;
+    else cost += (units * s <= slots ? 0 : 0.5 * units * (s * kFixed + rounds) / slots) + per + kFixed;
     if (best < 0 || cost < best) {
       best = cost;
       p.splits = int(s);
@@ -474,41 +552,61 @@ PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int max_len
   p.wblocks = accumulate ? int(std::min<int64_t>(64, (groups(max_len) * kPdGroup + 2047) / 2048)) : 0;
   p.join = p.splits > 1 || (accumulate && p.hgroups > 1);
   if (p.join) {
-    p.ml = pd_up(size_t(c.seqs) * heads * p.splits * 2 * sizeof(float));
-    p.po = p.splits > 1 ? pd_up(size_t(c.seqs) * heads * p.splits * c.hd * sizeof(float)) : 0;
+    p.ml = pd_up(size_t(rows) * heads * p.splits * 2 * sizeof(float));
+    p.po = p.splits > 1 ? pd_up(size_t(rows) * heads * p.splits * c.hd * sizeof(float)) : 0;
   }
   p.scores = accumulate ? pd_up(size_t(c.seqs) * heads * p.score_stride * sizeof(float)) : 0;
   return p;
 }
 
-template <int HD, bool BF>
+template <int HD, bool BF, bool MANY>
 cudaError_t pd_launch(const PdArgs &p, const PdPlan &plan, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<HD, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       PdRing<HD>::kBytes);
+  const auto kernel = paged_decode_kernel<HD, BF, MANY>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PdRing<HD>::kBytes);
   if (e != cudaSuccess) return e;
-  launch_pdl(paged_decode_kernel<HD, BF>, dim3(plan.splits, p.c.kv_heads * plan.hgroups, p.c.seqs), dim3(kPdWarps * 32),
-             PdRing<HD>::kBytes, st, p);
+  launch_pdl(kernel, dim3(plan.splits, p.c.kv_heads * plan.hgroups, p.c.seqs), dim3(kPdWarps * 32), PdRing<HD>::kBytes, st,
+             p);
+  const int outs = p.a.rep * (MANY ? p.max_rows : 1);
   if (plan.join)
-    launch_pdl(paged_join_kernel<HD, BF>, dim3(p.a.rep + plan.wblocks, p.c.kv_heads, p.c.seqs), dim3(kPdWarps * 32), 0, st,
-               p);
+    launch_pdl(paged_join_kernel<HD, BF>, dim3(outs + plan.wblocks, p.c.kv_heads, p.c.seqs), dim3(kPdWarps * 32), 0, st, p,
+               outs);
   return cudaGetLastError();
+}
+
+template <bool MANY>
+cudaError_t pd_run(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows, int max_rows, int max_len,
+                   bool accumulate, void *scratch, int sms, cudaStream_t st) {
+  const PdPlan plan = pd_plan(c, a.heads, a.window, a.first, rows, MANY, max_len, accumulate, sms);
+  uint8_t *base = static_cast<uint8_t *>(scratch);
+  const PdArgs p{c, a, plan.splits, plan.hgroups, accumulate, plan.score_stride, reinterpret_cast<float *>(base),
+                 reinterpret_cast<float *>(base + plan.ml), reinterpret_cast<float *>(base + plan.ml + plan.po), starts,
+                 rows, max_rows};
+  if (c.hd == 128) return c.bf16 ? pd_launch<128, true, MANY>(p, plan, st) : pd_launch<128, false, MANY>(p, plan, st);
+  return c.bf16 ? pd_launch<64, true, MANY>(p, plan, st) : pd_launch<64, false, MANY>(p, plan, st);
 }
 
 }  // namespace
 
 size_t paged_decode_scratch(const PagedView &c, int heads, int window, int first, int max_len, bool accumulate, int sms) {
-  const PdPlan p = pd_plan(c, heads, window, first, max_len, accumulate, sms);
+  const PdPlan p = pd_plan(c, heads, window, first, c.seqs, false, max_len, accumulate, sms);
   return p.ml + p.po + p.scores;
 }
 
 cudaError_t paged_decode(const PagedView &c, const PagedQuery &a, int max_len, bool accumulate, void *scratch, int sms,
                          cudaStream_t st) {
-  const PdPlan plan = pd_plan(c, a.heads, a.window, a.first, max_len, accumulate, sms);
-  uint8_t *base = static_cast<uint8_t *>(scratch);
-  const PdArgs p{c, a, plan.splits, plan.hgroups, accumulate, plan.score_stride, reinterpret_cast<float *>(base),
-                 reinterpret_cast<float *>(base + plan.ml), reinterpret_cast<float *>(base + plan.ml + plan.po)};
-  if (c.hd == 128) return c.bf16 ? pd_launch<128, true>(p, plan, st) : pd_launch<128, false>(p, plan, st);
-  return c.bf16 ? pd_launch<64, true>(p, plan, st) : pd_launch<64, false>(p, plan, st);
+  return pd_run<false>(c, a, nullptr, c.seqs, 1, max_len, accumulate, scratch, sms, st);
+}
+
+bool paged_few(const PagedView &c, int heads, int max_rows) { return int64_t(max_rows) * (heads / c.kv_heads) <= kPdFew; }
+
+size_t paged_few_scratch(const PagedView &c, int heads, int window, int first, int rows, int max_len, int sms) {
+  const PdPlan p = pd_plan(c, heads, window, first, rows, true, max_len, false, sms);
+  return p.ml + p.po;
+}
+
+cudaError_t paged_few_run(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows, int max_rows,
+                          int max_len, void *scratch, int sms, cudaStream_t st) {
+  return pd_run<true>(c, a, starts, rows, max_rows, max_len, false, scratch, sms, st);
 }
 
 }  // namespace hc
