@@ -56,7 +56,7 @@ __device__ __forceinline__ int sel_scan(int v, int *warps) {
   if (lane == 31) warps[warp] = x;
   __syncthreads();
   int before = 0;
-#pragma unroll
+#pragma unroll 4
   for (int w = 0; w < kSelThreads / 32; ++w) before += w < warp ? warps[w] : 0;
   __syncthreads();
   return before + x - v;
