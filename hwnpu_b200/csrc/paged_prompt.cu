@@ -23,14 +23,18 @@
 // long cache come out even. A block that a cut falls into is finished by a second kernel, which
 // joins the parts' (m, l, O) in order.
 //
-//   warps 0-3, 4-7  softmax of tile A, B: a thread owns a row. It reads the row's 128 scores from tensor
-//                   memory, keeps the running maximum and sum in float32, writes P back as 16-bit
-//                   values over the scores (a half of the slots at a time, so that P V of the first
-//                   runs beside the exponentials of the second), and at the end O / l to memory
+//   warps 0-3, 4-7  softmax of tile A, B: a thread owns a row. It takes 64 slots (a half of the tile) at
+//                   a time: reads the row's scores from tensor memory, keeps the running maximum and
+//                   sum in float32, writes P back as 16-bit values over the scores, and at the end O / l
+//                   to memory
 //   warp 8          copies the groups of K and V (cp.async.bulk.tensor, an mbarrier a ring stage)
 //   warps 9, 10     issue the MMAs of tile A, B: S = Q K^T (both operands in shared memory, 128-byte
 //                   swizzle), O += P V (P in tensor memory, V in shared memory, MN-major)
 //   warp 11         walks the CTA's part of the line, a block ahead of the others, and copies Q
+// The halves of a tile are two chains (S, softmax, P V, the same half's next S), so that the softmax has one half's
+// scores while the tensor cores have the other's P. An MMA of 64 slots takes nearly as long as one of 128 (59
+// clocks against 64), and it still pays: one chain a tile took 565 us for the 16,384-token prompt, two take 540 (904
+// TFLOP/s; copies alone bound it at 403), and 242 against 284 for ragged prompts in a window of 128.
 // The next block's K, V, Q and first scores are under way while a block's last tile and output are.
 //
 // Arithmetic. S and O are float32. P = exp2(S scale log2(e) - m) is rounded to the cache's type (the MMA
@@ -59,6 +63,7 @@ constexpr int kPpRows = 128;               // rows of a tile (the MMA's M)
 constexpr int kPpSlots = 128;              // slots of a tile
 constexpr int kPpGroup = 16;               // slots of a group (one TMA box, one K-step of P V)
 constexpr int kPpGroups = kPpSlots / kPpGroup;
+constexpr int kPpHalfGroups = kPpGroups / 2;  // of a half tile: the step of the softmax
 constexpr int kPpSoft = 256;               // threads of the softmax, one a row
 constexpr int kPpThreads = kPpSoft + 128;
 // Registers a thread: launched with 168 (65,536 / 384), then 208 for the softmax and 88 for the rest, which
@@ -136,35 +141,24 @@ __device__ __forceinline__ void pp_tma_v(uint32_t dst, const CUtensorMap *map, i
       "l"(map), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(tc_saddr(bar))
       : "memory");
 }
-// 128 columns of this warp's 32 lanes of tensor memory (a lane a row), waited for.
-__device__ __forceinline__ void pp_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+// 64 columns of this warp's 32 lanes of tensor memory (a lane a row), waited for.
+__device__ __forceinline__ void pp_ld64(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
       "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
-      "}, [%128];\n tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
-        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
-        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
-        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]),
-        "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]),
-        "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
-        "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]),
-        "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]),
-        "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]),
-        "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]),
-        "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]),
-        "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+        "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(taddr)
       : "memory");
 }
@@ -288,6 +282,9 @@ struct PpSpan {
 struct PpSeg : PpSpan {
   int i, h, j0, j1;
   int part;  // where unfinished rows go; -1: these are all the block's tiles, the output is written
+  __device__ __forceinline__ int halves() const {  // half tiles of 64 slots
+    return (min(groups, j1 * kPpGroups) - j0 * kPpGroups + kPpHalfGroups - 1) / kPpHalfGroups;
+  }
 };
 
 // The block whose first tiles a CTA has and whose last ones it has not: its parts are those of this
@@ -385,7 +382,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
   constexpr int kCopy = kPpSoft / 32, kMma = kCopy + 1, kWalk = kCopy + 3;  // warps
   extern __shared__ __align__(1024) uint8_t pp_sm[];  // the swizzle counts from 1,024-byte lines
   __shared__ uint64_t full[ST], empty[ST], vland, qfull, qempty, segfull[kPpSegs], segempty[kPpSegs];
-  __shared__ uint64_t sfull[2], pfull[2][2], ofull[2], ofree[2], exp_turn[2][4], done[2];
+  __shared__ uint64_t sfull[2][2], pfull[2][2], ofull[2], ofree[2], done[2];
   __shared__ PpSeg segs[kPpSegs];
   __shared__ PpShare share;
   __shared__ long long sums[kPpThreads / 32];
@@ -408,10 +405,10 @@ __global__ void __launch_bounds__(kPpThreads, 1)
       tc_bar_init(&segempty[s], kPpThreads / 32 - 1);  // every warp but the one that fills them
     }
     for (int x = 0; x < 2; ++x) {
-      tc_bar_init(&sfull[x], 1);
-      tc_bar_init(&pfull[x][0], 4);  // a half of the slots each
+      tc_bar_init(&sfull[x][0], 1);  // a half of the slots each
+      tc_bar_init(&sfull[x][1], 1);
+      tc_bar_init(&pfull[x][0], 4);
       tc_bar_init(&pfull[x][1], 4);
-      for (int w = 0; w < 4; ++w) tc_bar_init(&exp_turn[x][w], 1);
       tc_bar_init(&ofull[x], 1);
       tc_bar_init(&ofree[x], 4);
     }
@@ -613,29 +610,23 @@ __global__ void __launch_bounds__(kPpThreads, 1)
       const uint32_t idv = pp_idesc(BF, HD, true);
       const uint32_t neg = p.a.scale < 0.f ? 1u << 13 : 0u;  // the softmax takes |scale|
       const uint32_t idk = pp_idesc(BF, 0, false) | neg;
-      auto scores = [&](int at, int ng) {  // S = +-Q K^T of the stage's ng groups
-        const uint64_t kb = kd + at * (Sm::kTile >> 4);
+      auto scores = [&](int at, int half, int ng) {  // S = +-Q K^T of the ng groups of a half of the stage
+        const uint64_t kb = kd + at * (Sm::kTile >> 4) + half * ((kPpHalf / 2) >> 4);
         const uint32_t id = idk | uint32_t(ng * (kPpGroup >> 3)) << 17;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t off = ((k >> 2) * kPpHalf + (k & 3) * 32) >> 4;
-          tc_mma(ts, qd + off, kb + off, id, k > 0);
+          tc_mma(ts + 64 * half, qd + off, kb + off, id, k > 0);
         }
       };
       uint32_t vo[kPpGroups];  // V's groups in a stage, in units of 16 bytes
 #pragma unroll
       for (int g = 0; g < kPpGroups; ++g) vo[g] = pp_voff<HD>(g * kPpGroup, 0, p.box) >> 4;
-      auto values = [&](int at, int half, int ng, int add) {  // O += P V of a half's groups, as far as there are ng
+      auto values = [&](int at, int half, int ng, int add) {  // O += P V of the ng groups of a half
         const uint64_t vb = vd + at * (Sm::kTile >> 4);
-        if (half == 0) {
 #pragma unroll
-          for (int k = 0; k < kPpGroups / 2; ++k)
-            if (k < ng) pp_mma_ta(to, ts + 8 * k, vb + vo[k], idv, k > 0 ? 1 : add);
-        } else {
-#pragma unroll
-          for (int k = kPpGroups / 2; k < kPpGroups; ++k)
-            if (k < ng) pp_mma_ta(to, ts + 8 * k, vb + vo[k], idv, 1);
-        }
+        for (int k = 0; k < kPpHalfGroups; ++k)
+          if (k < ng) pp_mma_ta(to, ts + 64 * half + 8 * k, vb + vo[kPpHalfGroups * half + k], idv, k > 0 ? 1 : add);
       };
       int s = 0, turn = 0;  // the ring, as the copying warp fills it
       auto next = [&]() {
@@ -644,12 +635,12 @@ __global__ void __launch_bounds__(kPpThreads, 1)
           turn ^= 1;
         }
       };
-      int nq = 0, step = 0, blocks = 0;
+      int nq = 0, blocks = 0, ph[2] = {0, 0};  // ph: the halves' turns of P
       for (int k = 0;; ++k) {
         const PpSeg &sg = seg_get(k);
         if (*dead || sg.h < 0) break;
-        const int n = sg.j1 - sg.j0;
-        int left = sg.groups - sg.j0 * kPpGroups;  // groups from this tile on
+        const int n = sg.j1 - sg.j0, nu = sg.halves();
+        int left = sg.groups - sg.j0 * kPpGroups;  // groups from this half on
         const bool two = sg.t1 - sg.t0 > p.tokens;
         tc_arrive(&segempty[k % kPpSegs]);
         if (n <= 0) continue;
@@ -666,35 +657,39 @@ __global__ void __launch_bounds__(kPpThreads, 1)
         pp_wait(&qfull, (nq - 1) & 1, dead, 17);
         pp_wait(&full[s], turn, dead, 18);
         tc_fence_after();
-        scores(s, min(kPpGroups, left));
-        tc_commit(&sfull[x]);
+        scores(s, 0, min(kPpHalfGroups, left));
+        tc_commit(&sfull[x][0]);
+        if (nu > 1) {
+          scores(s, 1, min(kPpHalfGroups, left - kPpHalfGroups));
+          tc_commit(&sfull[x][1]);
+        }
         tc_commit(&empty[s]);
         if (n == 1) tc_commit(&qempty);
         next();
-        for (int v = 0; v < n; ++v, ++step) {
+        for (int v = 0; v < n; ++v) {
           const int sv = s;
           pp_wait(&full[sv], turn, dead, 19);
+          next();  // the next tile's keys
           if (v == 0 && blocks > 0) pp_wait(&ofree[x], (blocks - 1) & 1, dead, 20);
-          pp_wait(&pfull[x][0], step & 1, dead, 21);
-          tc_fence_after();
-          values(sv, 0, left, v > 0);
-          pp_wait(&pfull[x][1], step & 1, dead, 28);
-          tc_fence_after();
-          values(sv, 1, left, 1);
-          next();
-          left -= kPpGroups;
-          if (v + 1 < n) {
-            pp_wait(&full[s], turn, dead, 23);
-            scores(s, min(kPpGroups, left));
-            tc_commit(&sfull[x]);
-            tc_commit(&empty[sv]);
-            tc_commit(&empty[s]);
-            if (v + 2 == n) tc_commit(&qempty);
-            next();
-          } else {
-            tc_commit(&ofull[x]);
-            tc_commit(&empty[sv]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int u = 2 * v + half;
+            if (u >= nu) break;
+            pp_wait(&pfull[x][half], ph[half]++ & 1, dead, 21 + half);
+            tc_fence_after();
+            values(sv, half, min(kPpHalfGroups, left), u > 0);
+            left -= kPpHalfGroups;
+            if (u + 2 < nu) {
+              if (half == 0) pp_wait(&full[s], turn, dead, 23);
+              scores(s, half, min(kPpHalfGroups, left - kPpHalfGroups));
+            }
+            // S of half u + 2, or (for a rescale of half u + 1) only that P V of this half is done
+            tc_commit(u + 1 < nu ? &sfull[x][half] : &ofull[x]);
+            if (half == 1 || u + 1 == nu) tc_commit(&empty[sv]);
+            if (u + 2 < nu && (half == 1 || u + 3 == nu)) tc_commit(&empty[s]);
+            if (u + 3 == nu) tc_commit(&qempty);
           }
+          if (v + 1 < n) next();
           if (*dead) break;
         }
         ++blocks;
@@ -714,7 +709,8 @@ __global__ void __launch_bounds__(kPpThreads, 1)
     constexpr float kBias = BF ? 0.f : 7.f;
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + x * 128 + lanes, to = tmem + 256 + x * 128 + lanes;
-    int step = 0, done_blocks = 0, turns = 0;  // tiles, blocks and turns so far
+    int done_blocks = 0;  // so far
+    uint32_t sph = 0;     // bit h: the parity of half h's next S
     for (int k = 0;; ++k) {
       const PpSeg &sg = seg_get(k);
       if (__any_sync(0xffffffffu, *dead || sg.h < 0)) break;
@@ -730,25 +726,23 @@ __global__ void __launch_bounds__(kPpThreads, 1)
       const bool windowed = p.a.window > 0;
       const int wlo = windowed ? pos - p.a.window + 1 : -(1 << 30), wmax = windowed ? pmax - p.a.window + 1 : -(1 << 30);
       const int ga = sg.ga, b0 = sg.b0 - sg.ga, groups = sg.groups;
-      // The exponentials of the two tiles take turns, warp by warp (warps w and w + 4 share a scheduler): side by
-      // side they take twice as long each, and then both tiles wait for MMAs at the same time (575 us against
-      // 549 for the 16,384-token prompt). Blocks of few tiles end before that pays (257 us against 294 for
-      // ragged prompts in a window of 128).
-      const bool alternate = sg.t1 - sg.t0 > p.tokens && n >= kPpGroups;
       // groups [whole0, whole1) are seen by every row of the block: slots from wmax to pmin, in one run
       const int whole0 = max(b0 > 0 ? ga : 0, (max(wmax, 0) + kPpGroup - 1) / kPpGroup - b0);
       const int whole1 = (pmin + 1) / kPpGroup - b0;
       float m = -INFINITY, ref = 0.f, l = 0.f;  // m: of the scores as they are; ref: of exp2's argument
-      for (int v = 0; v < n; ++v, ++step) {
-        const int gb = g0 + v * kPpGroups;
-        const bool half_only = groups - gb <= kPpGroups / 2;  // a last tile with no more than a half
-        pp_wait(&sfull[x], step & 1, dead, 24);
+      const int nu = sg.halves();
+#pragma unroll 1
+      for (int u = 0; u < nu; ++u) {
+        const int half = u & 1, gb = g0 + kPpHalfGroups * u;
+        const uint32_t tsh = ts + 64 * half;
+        pp_wait(&sfull[x][half], (sph >> half) & 1, dead, 24);
+        sph ^= 1u << half;
         tc_fence_after();
-        if (!(gb >= whole0 && gb + kPpGroups <= whole1)) {
+        if (!(gb >= whole0 && gb + kPpHalfGroups <= whole1)) {
           // hidden scores, in tensor memory, a group at a time (a short loop: straight code for 128 columns was
           // fetched anew for every block); groups that all rows of the block see are left alone
 #pragma unroll 1
-          for (int g = 0; g < (half_only ? kPpGroups / 2 : kPpGroups); ++g) {
+          for (int g = 0; g < kPpHalfGroups; ++g) {
             const int gg = gb + g, s0 = gg < groups ? kPpGroup * (gg < ga ? gg : gg + b0) : (1 << 30);
             if (s0 + kPpGroup - 1 <= pmin && (s0 >= wmax || s0 + kPpGroup <= p.a.first)) continue;
             // the visible columns of the group: c <= hi and (c >= lo or c < fi)
@@ -757,22 +751,18 @@ __global__ void __launch_bounds__(kPpThreads, 1)
             const uint32_t see = ((1u << hi) - 1) & (~((1u << lo) - 1) | ((1u << fi) - 1));
             float y[16];
             uint32_t z[16];
-            tc_ld16(ts + 16 * g, y);
+            tc_ld16(tsh + 16 * g, y);
 #pragma unroll
             for (int c = 0; c < kPpGroup; ++c) z[c] = (see & (1u << c)) ? __float_as_uint(y[c]) : 0xff800000u;
-            pp_st16(ts + 16 * g, z);
+            pp_st16(tsh + 16 * g, z);
           }
           pp_wait_st();
         }
-        uint32_t s[128];
-        pp_ld128(ts, s);
-        if (half_only) {
-#pragma unroll
-          for (int c = 64; c < kPpSlots; ++c) s[c] = 0xff800000u;
-        }
+        uint32_t s[64];
+        pp_ld64(tsh, s);
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < kPpSlots; c += 2)
+        for (int c = 0; c < 64; c += 2)
           mx[(c >> 1) & 3] = pp_max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
         const float top = fmaxf(pp_max3(mx[0], mx[1], mx[2]), mx[3]);
         const bool move = (top - m) * scale2 > kPpLazy;
@@ -785,8 +775,10 @@ __global__ void __launch_bounds__(kPpThreads, 1)
             ref = nref;
             l *= f;
           }
-          if (v > 0) {
-            // O is complete up to the last tile: these scores were issued behind its product
+          if (u > 0) {
+            // O is complete up to the last half once the next half's S is: that was issued behind its product
+            pp_wait(&sfull[x][half ^ 1], (sph >> (half ^ 1)) & 1, dead, 30);
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
               float o[16];
@@ -798,39 +790,29 @@ __global__ void __launch_bounds__(kPpThreads, 1)
             }
           }
         }
-        if (alternate) {
-          if (x == 1) pp_wait(&exp_turn[1][warp & 3], turns & 1, dead, 29);
-          else if (turns > 0) pp_wait(&exp_turn[0][warp & 3], (turns - 1) & 1, dead, 29);
-          ++turns;
-        }
         uint64_t ls[2] = {0, 0};
         const uint64_t sc2 = pp_two(scale2, scale2), rf2 = pp_two(-ref, -ref);
+        uint32_t w[32];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (half == 1 && half_only) {
-            if (lane == 0) tc_arrive(&pfull[x][1]);
-            break;
-          }
-          uint32_t w[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const uint64_t x2 =
-                pp_fma2(pp_two(__uint_as_float(s[64 * half + 2 * c]), __uint_as_float(s[64 * half + 2 * c + 1])), sc2, rf2);
-            float2 e = pp_split(x2);
-            e.x = pp_exp2(e.x);
-            e.y = pp_exp2(e.y);
-            ls[c & 1] = pp_add2(ls[c & 1], pp_two(e.x, e.y));
-            w[c] = pp_pack<BF>(e.x, e.y);
-          }
-          pp_st32(ts + 32 * half, w);
-          pp_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) tc_arrive(&pfull[x][half]);
+        for (int c = 0; c < 32; ++c) {
+          const uint64_t x2 = pp_fma2(pp_two(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, rf2);
+          float2 e = pp_split(x2);
+          e.x = pp_exp2(e.x);
+          e.y = pp_exp2(e.y);
+          ls[c & 1] = pp_add2(ls[c & 1], pp_two(e.x, e.y));
+          w[c] = pp_pack<BF>(e.x, e.y);
         }
-        if (alternate && lane == 0) tc_arrive(&exp_turn[x ^ 1][warp & 3]);
+        pp_st32(tsh, w);
+        pp_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc_arrive(&pfull[x][half]);
         const float2 lsum = pp_split(pp_add2(ls[0], ls[1]));
         l += lsum.x + lsum.y;
+      }
+      if (nu > 1) {  // the turn that no further S came with
+        pp_wait(&sfull[x][nu & 1], (sph >> (nu & 1)) & 1, dead, 24);
+        sph ^= 1u << (nu & 1);
       }
       // The rows: O / l, or what a second kernel makes it of. O is read as an MMA's fragment, 16 rows and 32
       // columns at a time, and a quad's words are transposed, so that rows leave in runs of 64 bytes.
