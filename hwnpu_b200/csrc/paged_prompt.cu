@@ -17,7 +17,7 @@
 // spent on the slots between. Rows of an edge group that no row of the block sees are zeroed in shared
 // memory (values only: a hidden score is replaced, but 0 times a hidden NaN would not be 0).
 //
-// Work. One CTA an SM. All blocks of all heads and sequences, as many tiles long as they see (and one
+// Work. One CTA an SM, or two with head_dim 64. All blocks of all heads and sequences, as many tiles long as they see (and one
 // more for a block's start and end), lie one behind the other, and every CTA takes an equal part of that
 // line, read from the lengths on the device: ragged sequences, causal triangles and few rows over a
 // long cache come out even. A block that a cut falls into is finished by a second kernel, which
@@ -31,10 +31,10 @@
 //   warps 9, 10     issue the MMAs of tile A, B: S = Q K^T (both operands in shared memory, 128-byte
 //                   swizzle), O += P V (P in tensor memory, V in shared memory, MN-major)
 //   warp 11         walks the CTA's part of the line, a block ahead of the others, and copies Q
-// The halves of a tile are two chains (S, softmax, P V, the same half's next S), so that the softmax has one half's
-// scores while the tensor cores have the other's P. An MMA of 64 slots takes nearly as long as one of 128 (59
-// clocks against 64), and it still pays: one chain a tile took 565 us for the 16,384-token prompt, two take 540 (904
-// TFLOP/s; copies alone bound it at 403), and 242 against 284 for ragged prompts in a window of 128.
+// With head_dim 128 the halves of a tile are two chains (S, softmax, P V, the same half's next S), so that the softmax
+// has one half's scores while the tensor cores have the other's P. An MMA of 64 slots takes nearly as long as one
+// of 128 (59 clocks against 64), and it still pays: one chain a tile took 565 us for the 16,384-token prompt, two
+// take 533 (914 TFLOP/s; copies alone bound it at 403). With 64 there are two CTAs an SM instead.
 // The next block's K, V, Q and first scores are under way while a block's last tile and output are.
 //
 // Arithmetic. S and O are float32. P = exp2(S scale log2(e) - m) is rounded to the cache's type (the MMA
@@ -66,13 +66,9 @@ constexpr int kPpGroups = kPpSlots / kPpGroup;
 constexpr int kPpHalfGroups = kPpGroups / 2;  // of a half tile: the step of the softmax
 constexpr int kPpSoft = 256;               // threads of the softmax, one a row
 constexpr int kPpThreads = kPpSoft + 128;
-// Registers a thread: launched with 168 (65,536 / 384), then 208 for the softmax and 88 for the rest, which
-// adds up to the same (2 x 208 + 88 = 3 x 168).
-constexpr int kPpSoftRegs = 208, kPpRestRegs = 88;
 constexpr int kPpHalf = kPpRows * 128;     // bytes of 128 rows x 64 columns
 constexpr float kPpLazy = 8.f;
 constexpr float kPpLog2e = 1.4426950408889634f;
-constexpr uint32_t kPpTmem = 512;          // columns: S_A, S_B (128 each), O_A, O_B
 constexpr int kPpSegs = 4;                 // blocks the walking warp may be ahead
 constexpr int kPpMinPart = 4;              // least tiles of a CTA's part of the line
 
@@ -80,8 +76,18 @@ template <int HD>
 struct PpSmem {
   static constexpr int kHalves = HD / 64;
   static constexpr int kTile = kHalves * kPpHalf;  // Q of a tile, or K or V of 128 slots
-  static constexpr int kStages = HD == 128 ? 5 : 10;
-  static constexpr int kBytes = (2 + kStages) * kTile;  // 224 KB with head_dim 128: 3 KB are left
+  // CTAs an SM: tensor memory has room for one with head_dim 128, and for two with 64 when a tile has one half's
+  // scores at a time. Four tiles of one chain each then fill each other's gaps, a block's start and end among them:
+  // 186 us against 240 with two tiles of two chains for ragged prompts in a window of 128.
+  static constexpr int kCtas = HD == 128 ? 1 : 2;
+  static constexpr int kBufs = HD == 128 ? 2 : 1;  // halves of S a tile
+  static constexpr int kStages = HD == 128 ? 5 : 4;
+  static constexpr int kBytes = (2 + kStages) * kTile;  // 224 KB, or 96: 3 KB or 18 a CTA are left
+  static constexpr uint32_t kTmem = 2 * (64 * kBufs + HD);  // columns: S_A, S_B, O_A, O_B
+  // Scores a thread holds: all 64 of a half, or 32, read twice, where two CTAs leave it 80 registers. One CTA's 168
+  // (65,536 / 384) become 208 for the softmax and 88 for the rest, which adds up to the same (2 x 208 + 88 = 3 x 168).
+  static constexpr int kHeld = HD == 128 ? 64 : 32;
+  static constexpr int kSoftRegs = 208, kRestRegs = 88;
 };
 
 __device__ int pp_status_word;  // the first wait that ran out in any launch (0: none)
@@ -141,8 +147,8 @@ __device__ __forceinline__ void pp_tma_v(uint32_t dst, const CUtensorMap *map, i
       "l"(map), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(tc_saddr(bar))
       : "memory");
 }
-// 64 columns of this warp's 32 lanes of tensor memory (a lane a row), waited for.
-__device__ __forceinline__ void pp_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+// 64 or 32 columns of this warp's 32 lanes of tensor memory (a lane a row), waited for.
+__device__ __forceinline__ void pp_ld(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -162,7 +168,21 @@ __device__ __forceinline__ void pp_ld64(uint32_t taddr, uint32_t (&r)[64]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void pp_ld(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+      "}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void pp_st(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
@@ -172,7 +192,7 @@ __device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t (&r)[16])
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void pp_st(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -374,11 +394,11 @@ __device__ __forceinline__ void pp_share(const PpArgs &p, PpShare *sh, long long
 }
 
 template <int HD, bool BF>
-__global__ void __launch_bounds__(kPpThreads, 1)
+__global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
     paged_prompt_kernel(const PpArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const __grid_constant__ CUtensorMap qmap) {
   using Sm = PpSmem<HD>;
-  constexpr int ST = Sm::kStages;
+  constexpr int ST = Sm::kStages, NB = Sm::kBufs, CH = Sm::kHeld;
   constexpr int kCopy = kPpSoft / 32, kMma = kCopy + 1, kWalk = kCopy + 3;  // warps
   extern __shared__ __align__(1024) uint8_t pp_sm[];  // the swizzle counts from 1,024-byte lines
   __shared__ uint64_t full[ST], empty[ST], vland, qfull, qempty, segfull[kPpSegs], segempty[kPpSegs];
@@ -419,7 +439,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
   }
   if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_saddr(&tmem_base)),
-                 "r"(kPpTmem)
+                 "r"(Sm::kTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -440,7 +460,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
   };
 
   if (warp >= kPpSoft / 32) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpRestRegs));
+    if (Sm::kCtas == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sm::kRestRegs));
     // One elected thread a warp issues. (Issued by `lane == 0` instead, an MMA took 480 clocks of its warp beside
     // 16 busy ones, against 70: only elect.sync tells the compiler that one thread is left.)
     if (warp == kWalk) {
@@ -603,7 +623,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
       // The MMAs of tile A (warp kMma) or B (the next): a warp each, since a step's waits and commits take one
       // thread about as long as its MMAs take the tensor cores.
       const int x = warp - kMma;
-      const uint32_t ts = tmem + x * 128, to = tmem + 256 + x * 128;
+      const uint32_t ts = tmem + x * 64 * NB, to = tmem + 128 * NB + x * HD;
       // descriptors of the first K-step; the others differ in the address (units of 16 bytes)
       const uint64_t qd = pp_desc(tc_saddr(qsm + x * Sm::kTile), 16);
       const uint64_t kd = pp_desc(tc_saddr(ring), 16), vd = pp_desc(tc_saddr(ring), p.box * 128);
@@ -616,7 +636,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t off = ((k >> 2) * kPpHalf + (k & 3) * 32) >> 4;
-          tc_mma(ts + 64 * half, qd + off, kb + off, id, k > 0);
+          tc_mma(ts + 64 * (half % NB), qd + off, kb + off, id, k > 0);
         }
       };
       uint32_t vo[kPpGroups];  // V's groups in a stage, in units of 16 bytes
@@ -626,7 +646,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
         const uint64_t vb = vd + at * (Sm::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < kPpHalfGroups; ++k)
-          if (k < ng) pp_mma_ta(to, ts + 64 * half + 8 * k, vb + vo[kPpHalfGroups * half + k], idv, k > 0 ? 1 : add);
+          if (k < ng) pp_mma_ta(to, ts + 64 * (half % NB) + 8 * k, vb + vo[kPpHalfGroups * half + k], idv, k > 0 ? 1 : add);
       };
       int s = 0, turn = 0;  // the ring, as the copying warp fills it
       auto next = [&]() {
@@ -659,12 +679,17 @@ __global__ void __launch_bounds__(kPpThreads, 1)
         tc_fence_after();
         scores(s, 0, min(kPpHalfGroups, left));
         tc_commit(&sfull[x][0]);
-        if (nu > 1) {
+        if (NB == 2 && nu > 1) {
           scores(s, 1, min(kPpHalfGroups, left - kPpHalfGroups));
           tc_commit(&sfull[x][1]);
         }
-        tc_commit(&empty[s]);
-        if (n == 1) tc_commit(&qempty);
+        if (nu <= NB) {
+          tc_commit(&empty[s]);
+          tc_commit(&qempty);
+        } else if (NB == 2) {
+          tc_commit(&empty[s]);
+        }
+        int sk = s;  // the stage of this tile's keys
         next();
         for (int v = 0; v < n; ++v) {
           const int sv = s;
@@ -673,22 +698,26 @@ __global__ void __launch_bounds__(kPpThreads, 1)
           if (v == 0 && blocks > 0) pp_wait(&ofree[x], (blocks - 1) & 1, dead, 20);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int u = 2 * v + half;
+            const int u = 2 * v + half, buf = half % NB;
             if (u >= nu) break;
-            pp_wait(&pfull[x][half], ph[half]++ & 1, dead, 21 + half);
+            pp_wait(&pfull[x][buf], ph[buf]++ & 1, dead, 21 + half);
             tc_fence_after();
             values(sv, half, min(kPpHalfGroups, left), u > 0);
             left -= kPpHalfGroups;
-            if (u + 2 < nu) {
-              if (half == 0) pp_wait(&full[s], turn, dead, 23);
-              scores(s, half, min(kPpHalfGroups, left - kPpHalfGroups));
+            // S of half u + NB, which takes this one's place
+            const bool here = NB == 1 && half == 0;  // it is of this tile
+            const int su = here ? sk : s;
+            if (u + NB < nu) {
+              if (half == 2 - NB) pp_wait(&full[s], turn, dead, 23);  // its first half
+              scores(su, (half + NB) & 1, min(kPpHalfGroups, left - (NB - 1) * kPpHalfGroups));
             }
-            // S of half u + 2, or (for a rescale of half u + 1) only that P V of this half is done
-            tc_commit(u + 1 < nu ? &sfull[x][half] : &ofull[x]);
+            // with two halves of S, the last but one turn tells only (for a rescale) that P V of this half is done
+            tc_commit(u + 1 < nu ? &sfull[x][buf] : &ofull[x]);
             if (half == 1 || u + 1 == nu) tc_commit(&empty[sv]);
-            if (u + 2 < nu && (half == 1 || u + 3 == nu)) tc_commit(&empty[s]);
-            if (u + 3 == nu) tc_commit(&qempty);
+            if (u + NB < nu && (((half + NB) & 1) == 1 || u + NB + 1 == nu)) tc_commit(&empty[su]);
+            if (u + NB + 1 == nu) tc_commit(&qempty);
           }
+          sk = s;
           if (v + 1 < n) next();
           if (*dead) break;
         }
@@ -699,7 +728,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
       tc_wait(&done[x], 0, &pp_status_word, 25);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpSoftRegs));
+    if (Sm::kCtas == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sm::kSoftRegs));
     const int x = warp >> 2, row = threadIdx.x & 127;
     // row / rep of a row below 128, rep at most 128: 65,536 / rep rounded up is close enough to be exact
     const int rep = p.a.rep, recip = (65536 + rep - 1) / rep;
@@ -708,7 +737,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
     const float scale2 = fmaxf(fabsf(p.a.scale) * kPpLog2e, 1e-37f);
     constexpr float kBias = BF ? 0.f : 7.f;
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + x * 128 + lanes, to = tmem + 256 + x * 128 + lanes;
+    const uint32_t ts = tmem + x * 64 * NB + lanes, to = tmem + 128 * NB + x * HD + lanes;
     int done_blocks = 0;  // so far
     uint32_t sph = 0;     // bit h: the parity of half h's next S
     for (int k = 0;; ++k) {
@@ -733,10 +762,10 @@ __global__ void __launch_bounds__(kPpThreads, 1)
       const int nu = sg.halves();
 #pragma unroll 1
       for (int u = 0; u < nu; ++u) {
-        const int half = u & 1, gb = g0 + kPpHalfGroups * u;
-        const uint32_t tsh = ts + 64 * half;
-        pp_wait(&sfull[x][half], (sph >> half) & 1, dead, 24);
-        sph ^= 1u << half;
+        const int buf = u % NB, gb = g0 + kPpHalfGroups * u;
+        const uint32_t tsh = ts + 64 * buf;
+        pp_wait(&sfull[x][buf], (sph >> buf) & 1, dead, 24);
+        sph ^= 1u << buf;
         tc_fence_after();
         if (!(gb >= whole0 && gb + kPpHalfGroups <= whole1)) {
           // hidden scores, in tensor memory, a group at a time (a short loop: straight code for 128 columns was
@@ -754,16 +783,19 @@ __global__ void __launch_bounds__(kPpThreads, 1)
             tc_ld16(tsh + 16 * g, y);
 #pragma unroll
             for (int c = 0; c < kPpGroup; ++c) z[c] = (see & (1u << c)) ? __float_as_uint(y[c]) : 0xff800000u;
-            pp_st16(tsh + 16 * g, z);
+            pp_st(tsh + 16 * g, z);
           }
           pp_wait_st();
         }
-        uint32_t s[64];
-        pp_ld64(tsh, s);
+        uint32_t s[CH];
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 64; c += 2)
-          mx[(c >> 1) & 3] = pp_max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        for (int part = 0; part < 64; part += CH) {
+          pp_ld(tsh + part, s);
+#pragma unroll
+          for (int c = 0; c < CH; c += 2)
+            mx[(c >> 1) & 3] = pp_max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        }
         const float top = fmaxf(pp_max3(mx[0], mx[1], mx[2]), mx[3]);
         const bool move = (top - m) * scale2 > kPpLazy;
         if (__any_sync(0xffffffffu, move)) {
@@ -776,9 +808,12 @@ __global__ void __launch_bounds__(kPpThreads, 1)
             l *= f;
           }
           if (u > 0) {
-            // O is complete up to the last half once the next half's S is: that was issued behind its product
-            pp_wait(&sfull[x][half ^ 1], (sph >> (half ^ 1)) & 1, dead, 30);
-            tc_fence_after();
+            // O has to be complete up to the last half: this S was issued behind its product, or with two of
+            // them the next half's S
+            if (NB == 2) {
+              pp_wait(&sfull[x][buf ^ 1], (sph >> (buf ^ 1)) & 1, dead, 30);
+              tc_fence_after();
+            }
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
               float o[16];
@@ -786,31 +821,35 @@ __global__ void __launch_bounds__(kPpThreads, 1)
               tc_ld16(to + c, o);
 #pragma unroll
               for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
-              pp_st16(to + c, w);
+              pp_st(to + c, w);
             }
           }
         }
         uint64_t ls[2] = {0, 0};
         const uint64_t sc2 = pp_two(scale2, scale2), rf2 = pp_two(-ref, -ref);
-        uint32_t w[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const uint64_t x2 = pp_fma2(pp_two(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, rf2);
-          float2 e = pp_split(x2);
-          e.x = pp_exp2(e.x);
-          e.y = pp_exp2(e.y);
-          ls[c & 1] = pp_add2(ls[c & 1], pp_two(e.x, e.y));
-          w[c] = pp_pack<BF>(e.x, e.y);
+        for (int part = 0; part < 64; part += CH) {
+          if (CH < 64) pp_ld(tsh + part, s);  // (part's P lies over scores that have been read)
+          uint32_t w[CH / 2];
+#pragma unroll
+          for (int c = 0; c < CH / 2; ++c) {
+            const uint64_t x2 = pp_fma2(pp_two(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, rf2);
+            float2 e = pp_split(x2);
+            e.x = pp_exp2(e.x);
+            e.y = pp_exp2(e.y);
+            ls[c & 1] = pp_add2(ls[c & 1], pp_two(e.x, e.y));
+            w[c] = pp_pack<BF>(e.x, e.y);
+          }
+          pp_st(tsh + part / 2, w);
         }
-        pp_st32(tsh, w);
         pp_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc_arrive(&pfull[x][half]);
+        if (lane == 0) tc_arrive(&pfull[x][buf]);
         const float2 lsum = pp_split(pp_add2(ls[0], ls[1]));
         l += lsum.x + lsum.y;
       }
-      if (nu > 1) {  // the turn that no further S came with
+      if (NB == 2 && nu > 1) {  // the turn that no further S came with
         pp_wait(&sfull[x][nu & 1], (sph >> (nu & 1)) & 1, dead, 24);
         sph ^= 1u << (nu & 1);
       }
@@ -887,7 +926,7 @@ __global__ void __launch_bounds__(kPpThreads, 1)
   __syncthreads();
   if (warp == kMma) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPpTmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sm::kTmem) : "memory");
   }
 }
 
@@ -997,12 +1036,13 @@ PpPlan pp_plan(const PagedView &c, int heads, int window, int first, int rows, i
   // before it, so short windows take small ones.
   p.box = kPpGroup;
   while (p.box < kPpSlots && 2 * p.box <= (1 << c.shift) && (window == 0 || 16 * p.box <= window)) p.box *= 2;
-  // one CTA an SM, or fewer when the longest line the sizes allow has fewer parts of kPpMinPart tiles
+  // one CTA an SM (two), or fewer when the longest line the sizes allow has fewer parts of kPpMinPart tiles
   int64_t see = max_len;
   if (window > 0) see = std::min<int64_t>(see, int64_t(window) + first + 2 * p.tokens + 2 * p.box);
   const int64_t tiles = (see + kPpSlots - 1) / kPpSlots + 1;
+  const int slots = sms * (c.hd == 128 ? PpSmem<128>::kCtas : PpSmem<64>::kCtas);
   const double line = double(p.blocks) * c.kv_heads * c.seqs * double(tiles);
-  p.ctas = int(std::max(1.0, std::min(double(sms), line / kPpMinPart + 1.0)));
+  p.ctas = int(std::max(1.0, std::min(double(slots), line / kPpMinPart + 1.0)));
   if (p.ctas > 1) {
     p.heads_bytes = (size_t(p.ctas) * sizeof(PpHead) + 255) / 256 * 256;
     p.ml = (size_t(2) * p.ctas * p.slot_rows * sizeof(float2) + 255) / 256 * 256;
