@@ -10,20 +10,28 @@
 namespace hc {
 
 // Launches k on st with programmatic stream serialization (device.cuh's pdl_trigger/pdl_wait): the
-// kernel may start while the one before it in the stream finishes.
+// kernel may start while the one before it in the stream finishes. cluster: CTAs of a cluster, along x.
 template <typename... KArgs, typename... Args>
-void launch_pdl(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
+void launch_pdl_cluster(void (*k)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t st,
+                        Args &&...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = unsigned(cluster);
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...);
+}
+template <typename... KArgs, typename... Args>
+void launch_pdl(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
+  launch_pdl_cluster(k, grid, block, 1, smem, st, std::forward<Args>(args)...);
 }
 
 

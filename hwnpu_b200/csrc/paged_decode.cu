@@ -25,8 +25,8 @@
 //                rounding left of P (rounded in its turn), so that the weights carry 16 bits or more
 //                at no further MMA; B is V by ldmatrix.trans. O is float32
 // Of several tokens both halves of A are rows, and the weights are rounded to the cache's type once.
-// The four warps' (m, l, O) are joined in shared memory, the splits' by a second kernel, both in a
-// fixed order. With `accumulate` the scores are kept in scratch (float32) and the visible slots' weights
+// The four warps' (m, l, O) are joined in shared memory, the splits' by a second kernel or, up to 8 of them,
+// by their cluster over distributed shared memory, all in a fixed order. With `accumulate` the scores are kept in scratch (float32) and the visible slots' weights
 // exp2(S - m) / l are summed over the heads once m and l are known.
 #include <cuda_bf16.h>
 
@@ -44,6 +44,7 @@ constexpr int kPdGroup = 16;   // slots of a group
 constexpr int kPdHeads = 8;    // query heads a CTA
 constexpr int kPdMaxSplits = 256;
 constexpr int kPdFew = 16;     // rows of several tokens a CTA
+constexpr int kPdCluster = 8;  // splits that a cluster joins
 constexpr float kPdLazy = 8.f;  // log2 of how far a score may pass the running maximum
 constexpr float kPdLog2e = 1.4426950408889634f;
 
@@ -66,6 +67,18 @@ __device__ __forceinline__ uint32_t pd_saddr(const void *p) {
 __device__ __forceinline__ void pd_cp16(uint32_t dst, const void *src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+// Two floats at addr of the cluster's CTA `rank`.
+__device__ __forceinline__ float2 pd_peer(uint32_t addr, int rank) {
+  float2 v;
+  asm volatile(
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %2, %3;\n ld.shared::cluster.v2.f32 {%0, %1}, [a];\n}\n"
+      : "=f"(v.x), "=f"(v.y)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+__device__ __forceinline__ void pd_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pd_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pd_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void pd_wait() {
@@ -137,7 +150,7 @@ struct PdArgs {
   PagedView c;
   PagedQuery a;
   int splits, hgroups;
-  bool accumulate;
+  bool accumulate, cluster;  // cluster: the splits of a row are one, and join themselves
   int64_t score_stride;  // scores a head keeps in scratch
   float *part_ml;        // [rows][heads][splits][2]: m (log2 units) and l
   float *part_o;         // [rows][heads][splits][hd], not divided by l
@@ -194,7 +207,8 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
   constexpr float kBias = BF ? 0.f : 7.f;
   extern __shared__ __align__(128) uint8_t pd_buf[];
   __shared__ float sm_m[kPdWarps][ROWS], sm_l[kPdWarps][ROWS];
-  __shared__ float2 sm_ml[ROWS];
+  __shared__ float2 sm_ml[ROWS], cl_ml[ROWS];
+  __shared__ float sm_f[kPdFew][kPdCluster];
   pdl_trigger();
   pdl_wait();
   const PagedView &c = p.c;
@@ -205,8 +219,8 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
   const PdSpan sp = rw.span(p);
   const int per = sp.per(p.splits);
   const int g0 = split * per, g1 = min(sp.groups, g0 + per);
-  if (g0 >= g1 && split > 0) return;
-  const bool alone = sp.groups <= per;  // this CTA has the whole row
+  const bool alone = sp.groups <= per;  // one CTA has the whole row
+  if (g0 >= g1 && split > 0 && (alone || !p.cluster)) return;
   const int rep = p.a.rep, head0 = h * rep + hg * kPdHeads;
   const int nrows = MANY ? rw.count * rep : min(kPdHeads, rep - hg * kPdHeads);
   // groups that every row sees: below the first one's slot, from the last one's window on
@@ -372,7 +386,8 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
   __syncthreads();  // every warp is done with its ring
 
   // join the warps: [warp][row][hd] float32 in the ring's memory
-  float *po = reinterpret_cast<float *>(pd_buf);
+  float *po = reinterpret_cast<float *>(pd_buf), *cl_o = po + kPdWarps * ROWS * HD;
+  static_assert((kPdWarps + 1) * ROWS * HD * sizeof(float) <= Ring::kBytes, "the joined rows lie behind the warps'");
 #pragma unroll
   for (int b = 0; b < HALVES; ++b) {
     l[b] += __shfl_xor_sync(0xffffffffu, l[b], 1);
@@ -413,16 +428,67 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
       const float inv = ll > 0.f ? 1.f / ll : 0.f;
       *reinterpret_cast<uint32_t *>(p.a.o + row * p.a.o_row + hq * p.a.o_head + d) = pd_pack<BF>(vx * inv, vy * inv);
       if (d == 0) sm_ml[r] = make_float2(ref, inv);
+    } else if (p.cluster) {
+      *reinterpret_cast<float2 *>(cl_o + r * HD + d) = make_float2(vx, vy);
+      if (d == 0) cl_ml[r] = make_float2(mm, ll);
     } else {
       const int64_t at = (int64_t(row) * p.a.heads + hq) * p.splits + split;
       *reinterpret_cast<float2 *>(p.part_o + at * HD + d) = make_float2(vx, vy);
       if (d == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(mm, ll);
     }
   }
-  if (!MANY && p.accumulate && alone && p.hgroups == 1) {
-    __syncthreads();
-    pd_add_weights(p, sp, i, h, 0, sp.groups, sm_ml);
+  if (alone) {
+    if (!MANY && p.accumulate && p.hgroups == 1) {
+      __syncthreads();
+      pd_add_weights(p, sp, i, h, 0, sp.groups, sm_ml);
+    }
+    return;
   }
+  if (!p.cluster) return;
+  // The cluster's CTAs have the splits of these rows: what each split counts for (8 lanes a row), then a share of the
+  // output each, and the weights of the own slots.
+  __syncwarp();
+  pd_cluster_arrive();
+  pd_cluster_wait();
+  {
+    static_assert(kPdFew * kPdCluster == kPdWarps * 32, "a thread a row and split");
+    const int r = threadIdx.x / kPdCluster, s = threadIdx.x % kPdCluster;
+    const bool there = r < nrows && s < p.splits;
+    const float2 ml = there ? pd_peer(pd_saddr(&cl_ml[min(r, ROWS - 1)]), s) : make_float2(-INFINITY, 0.f);
+    const float sink =
+        p.a.sinks && r < nrows ? p.a.sinks[head0 + (MANY ? r % rep : r)] * kPdLog2e : -INFINITY;
+    float mm = fmaxf(ml.x, sink);
+#pragma unroll
+    for (int y = 1; y < kPdCluster; y <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, y));
+    const float ref = mm == -INFINITY ? 0.f : mm, f = exp2f(ml.x - ref);
+    float ll = f * ml.y;
+#pragma unroll
+    for (int y = 1; y < kPdCluster; y <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, y);
+    ll += exp2f(sink - ref);
+    const float inv = ll > 0.f ? 1.f / ll : 0.f;
+    sm_f[r][s] = f * inv;
+    if (s == 0 && r < nrows) sm_ml[r] = make_float2(ref, inv);
+  }
+  __syncthreads();
+  for (int u = split * (kPdWarps * 32) + threadIdx.x; u < nrows * (HD / 2); u += p.splits * (kPdWarps * 32)) {
+    const int r = u / (HD / 2), d = 2 * (u % (HD / 2)), tok = MANY ? r / rep : 0;
+    const uint32_t at = pd_saddr(cl_o + r * HD + d);
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int s = 0; s < kPdCluster; ++s) {
+      if (s >= p.splits) break;
+      const float2 v = pd_peer(at, s);
+      x = fmaf(sm_f[r][s], v.x, x);
+      y = fmaf(sm_f[r][s], v.y, y);
+    }
+    *reinterpret_cast<uint32_t *>(p.a.o + (rw.row0 + tok) * p.a.o_row + (head0 + r - tok * rep) * p.a.o_head + d) =
+        pd_pack<BF>(x, y);
+  }
+  __syncwarp();
+  pd_cluster_arrive();
+  if (!MANY && p.accumulate) pd_add_weights(p, sp, i, h, g0, g1, sm_ml);
+  __syncwarp();
+  pd_cluster_wait();  // no CTA ends while another reads its rows
 }
 
 // m (log2 units) and 1 / l of a query head over all its splits and its sink; by one warp.
@@ -512,7 +578,7 @@ struct PdPlan {
   int splits, hgroups, wblocks;
   int64_t score_stride;
   size_t ml, po, scores;  // bytes
-  bool join;
+  bool cluster, join;     // the splits are joined by their cluster; by a second kernel
 };
 
 size_t pd_up(size_t n) { return (n + 255) / 256 * 256; }
@@ -525,22 +591,29 @@ PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int rows, b
   auto groups = [&](int len) -> int64_t {
     const int64_t all = (int64_t(len) + kPdGroup - 1) / kPdGroup;
     if (window == 0) return all;
-    return std::min<int64_t>(all, (int64_t(first) + kPdGroup - 1) / kPdGroup + (int64_t(window) + (few ? kPdFew : 0) + kPdGroup - 1) / kPdGroup + 1);
+    const int64_t run = int64_t(window) + (few ? kPdFew : 0);
+    return std::min<int64_t>(all, (int64_t(first) + kPdGroup - 1) / kPdGroup + (run + kPdGroup - 1) / kPdGroup + 1);
   };
   // The number of splits that ends soonest, in rounds (a group a warp) a CTA walks, its start and its join counted
-  // as kFixed rounds and the second kernel as as many. One sequence: waves of equal CTAs over the SMs. Several,
-  // whose lengths the host does not know: where not all CTAs fit at once, all rounds (half of what max_len allows)
-  // over the SMs, and then the CTA that ends last, so that a long sequence among short ones is cut (64 sequences of up to 8,200 slots
-  // took 300 us uncut).
-  constexpr double kFixed = 6;
-  const int64_t units = int64_t(c.seqs) * c.kv_heads * p.hgroups, slots = int64_t(sms) * (c.hd == 128 ? PdRing<128>::kCtas : PdRing<64>::kCtas);
+  // as kFixed rounds, the second kernel as as many. Up to 8 splits that fit at once are clusters, which join their
+  // own rows (kJoin rounds): 5 rows each of 8 sequences of 500 to 2,100 slots take 18.2 us so, 19.7 with the
+  // second kernel. Clusters that have to wait for room cost more than it (244 us against 206 for 64 sequences of
+  // up to 8,200 slots). One sequence: waves of equal CTAs over the SMs. Several, whose lengths the host does not
+  // know: where not all CTAs fit at once, all rounds (half of what max_len allows) over the SMs, and then the CTA
+  // that ends last, so that a long sequence among short ones is cut (those 64 took 300 us uncut).
+  const int64_t units = int64_t(c.seqs) * c.kv_heads * p.hgroups;
+  const int64_t slots = int64_t(sms) * (c.hd == 128 ? PdRing<128>::kCtas : PdRing<64>::kCtas);
+  constexpr double kFixed = 6, kJoin = 2;
+  auto joins = [&](int64_t s) {  // with hgroups a CTA does not have all the heads that give weights
+    return s <= kPdCluster && units * s <= slots && (!accumulate || p.hgroups == 1);
+  };
   const int64_t rounds = std::max<int64_t>(1, (groups(max_len) + kPdWarps - 1) / kPdWarps);
   double best = -1;
   p.splits = 1;
   for (int64_t s = 1; s <= std::min<int64_t>(rounds, kPdMaxSplits); ++s) {
     const int64_t per = (rounds + s - 1) / s;
     if ((rounds + per - 1) / per != s) continue;
-    double cost = s > 1 ? kFixed : 0;
+    double cost = s == 1 ? 0 : joins(s) ? kJoin : kFixed;
     if (c.seqs == 1) cost += double((units * s + slots - 1) / slots) * (per + kFixed);
     else cost += (units * s <= slots ? 0 : 0.5 * units * (s * kFixed + rounds) / slots) + per + kFixed;
     if (best < 0 || cost < best) {
@@ -550,7 +623,8 @@ PdPlan pd_plan(const PagedView &c, int heads, int window, int first, int rows, b
   }
   p.score_stride = accumulate ? groups(c.cap) * kPdGroup : 0;
   p.wblocks = accumulate ? int(std::min<int64_t>(64, (groups(max_len) * kPdGroup + 2047) / 2048)) : 0;
-  p.join = p.splits > 1 || (accumulate && p.hgroups > 1);
+  p.cluster = p.splits > 1 && joins(p.splits);
+  p.join = (p.splits > 1 && !p.cluster) || (accumulate && p.hgroups > 1);
   if (p.join) {
     p.ml = pd_up(size_t(rows) * heads * p.splits * 2 * sizeof(float));
     p.po = p.splits > 1 ? pd_up(size_t(rows) * heads * p.splits * c.hd * sizeof(float)) : 0;
@@ -564,8 +638,8 @@ cudaError_t pd_launch(const PdArgs &p, const PdPlan &plan, cudaStream_t st) {
   const auto kernel = paged_decode_kernel<HD, BF, MANY>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PdRing<HD>::kBytes);
   if (e != cudaSuccess) return e;
-  launch_pdl(kernel, dim3(plan.splits, p.c.kv_heads * plan.hgroups, p.c.seqs), dim3(kPdWarps * 32), PdRing<HD>::kBytes, st,
-             p);
+  launch_pdl_cluster(kernel, dim3(plan.splits, p.c.kv_heads * plan.hgroups, p.c.seqs), dim3(kPdWarps * 32),
+                     plan.cluster ? plan.splits : 1, PdRing<HD>::kBytes, st, p);
   const int outs = p.a.rep * (MANY ? p.max_rows : 1);
   if (plan.join)
     launch_pdl(paged_join_kernel<HD, BF>, dim3(outs + plan.wblocks, p.c.kv_heads, p.c.seqs), dim3(kPdWarps * 32), 0, st, p,
@@ -578,7 +652,7 @@ cudaError_t pd_run(const PagedView &c, const PagedQuery &a, const int32_t *start
                    bool accumulate, void *scratch, int sms, cudaStream_t st) {
   const PdPlan plan = pd_plan(c, a.heads, a.window, a.first, rows, MANY, max_len, accumulate, sms);
   uint8_t *base = static_cast<uint8_t *>(scratch);
-  const PdArgs p{c, a, plan.splits, plan.hgroups, accumulate, plan.score_stride, reinterpret_cast<float *>(base),
+  const PdArgs p{c, a, plan.splits, plan.hgroups, accumulate, plan.cluster, plan.score_stride, reinterpret_cast<float *>(base),
                  reinterpret_cast<float *>(base + plan.ml), reinterpret_cast<float *>(base + plan.ml + plan.po), starts,
                  rows, max_rows};
   if (c.hd == 128) return c.bf16 ? pd_launch<128, true, MANY>(p, plan, st) : pd_launch<128, false, MANY>(p, plan, st);
