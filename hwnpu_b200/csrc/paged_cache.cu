@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
   extern __shared__ uint32_t sel_keys[];
   __shared__ int hist[kSelBins];
   __shared__ int warps[kSelThreads / 32];
-  __shared__ int sh_digit, sh_above;
+  __shared__ int sh_digit, sh_above, sh_count;
   pdl_trigger();
   pdl_wait();
   const int h = blockIdx.x, i = blockIdx.y, tid = threadIdx.x;
@@ -119,12 +119,15 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
       const bool upper = above + n0 >= need;
       sh_digit = upper ? d0 : d0 - 1;
       sh_above = above + (upper ? 0 : n0);
+      sh_count = upper ? n0 : n1;
     }
     __syncthreads();
     prefix |= uint32_t(sh_digit) << shift;
     known |= ((1u << bits) - 1) << shift;
     need -= sh_above;
+    const bool all = sh_count == need;  // every key with this prefix stays: the bits below do not matter
     __syncthreads();
+    if (all) break;
   }
   // runs of an odd number of candidates a thread: no two lanes on one bank
   const int run = ((cand + kSelThreads - 1) / kSelThreads) | 1;
