@@ -10,27 +10,48 @@
 namespace hc {
 namespace {
 
-// One thread a 16-byte piece of a row's key and of its value; CH pieces a row.
+// One thread a 16-byte piece of kAppendRows (row, head)s' keys and of their values, CH pieces a row. All pieces are on
+// their way while the rows' places are looked up (row, then block table: two loads that wait for one another).
+// Bound by HBM once there are enough rows: 75 MB (9,000 rows of 8 heads of 128) take 16.3 us, 4.6 TB/s; with 1 row a
+// thread 17.2, with 4 18.1.
+constexpr int kAppendRows = 2;
 template <int CH>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, const uint16_t *__restrict__ k,
                                                            const uint16_t *__restrict__ v, int64_t k_row,
                                                            int64_t k_head, int64_t v_row, int64_t v_head,
                                                            const int32_t *__restrict__ seq,
                                                            const int32_t *__restrict__ slot, int rows) {
-  const int64_t u = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int ch = int(u % CH);
-  const int64_t rh = u / CH;
-  if (rh >= int64_t(rows) * c.kv_heads) return;
-  const int r = int(rh / c.kv_heads), h = int(rh % c.kv_heads);
-  const int i = seq[r], j = slot[r];
-  if (unsigned(i) >= unsigned(c.seqs) || unsigned(j) >= unsigned(c.cap)) return;
-  const int64_t at = paged_row(c, i, h, j);
-  if (at < 0) return;
-  const uint4 kk = *reinterpret_cast<const uint4 *>(k + r * k_row + h * k_head + 8 * ch);
-  const uint4 vv = *reinterpret_cast<const uint4 *>(v + r * v_row + h * v_head + 8 * ch);
-  *reinterpret_cast<uint4 *>(c.k + at + 8 * ch) = kk;
-  *reinterpret_cast<uint4 *>(c.v + at + 8 * ch) = vv;
-  if (c.weights && ch == 0) c.weights[(int64_t(i) * c.kv_heads + h) * c.cap + j] = 0.f;
+  const int ch = threadIdx.x % CH;
+  const int64_t first = int64_t(blockIdx.x) * (256 / CH * kAppendRows) + threadIdx.x / CH;
+  uint4 kk[kAppendRows], vv[kAppendRows];
+  int i[kAppendRows], j[kAppendRows], h[kAppendRows];
+#pragma unroll
+  for (int u = 0; u < kAppendRows; ++u) {
+    const int64_t rh = first + u * (256 / CH);
+    const bool there = rh < int64_t(rows) * c.kv_heads;
+    const int r = there ? int(rh / c.kv_heads) : 0;
+    h[u] = there ? int(rh % c.kv_heads) : 0;
+    i[u] = there ? seq[r] : -1;
+    j[u] = there ? slot[r] : -1;
+    kk[u] = vv[u] = make_uint4(0, 0, 0, 0);
+    if (there) {
+      kk[u] = *reinterpret_cast<const uint4 *>(k + r * k_row + h[u] * k_head + 8 * ch);
+      vv[u] = *reinterpret_cast<const uint4 *>(v + r * v_row + h[u] * v_head + 8 * ch);
+    }
+  }
+  int64_t at[kAppendRows];
+#pragma unroll
+  for (int u = 0; u < kAppendRows; ++u) {
+    const bool in = unsigned(i[u]) < unsigned(c.seqs) && unsigned(j[u]) < unsigned(c.cap);
+    at[u] = in ? paged_row(c, i[u], h[u], j[u]) : -1;
+  }
+#pragma unroll
+  for (int u = 0; u < kAppendRows; ++u) {
+    if (at[u] < 0) continue;
+    *reinterpret_cast<uint4 *>(c.k + at[u] + 8 * ch) = kk[u];
+    *reinterpret_cast<uint4 *>(c.v + at[u] + 8 * ch) = vv[u];
+    if (c.weights && ch == 0) c.weights[(int64_t(i[u]) * c.kv_heads + h[u]) * c.cap + j[u]] = 0.f;
+  }
 }
 
 // A weight as a key whose unsigned order is the order evict keeps by: NaN lowest, -0 as +0.
@@ -152,8 +173,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
 
 // Copies the kept rows: a thread has a 16-byte piece of kCopyRows rows, keys and values, all loaded before the
 // first is stored. Bound by HBM: 4,096 rows a head of 16 sequences of 8 heads of 128, 270 MB read and as much
-// written, take 93 us (5.3 TB/s).
-constexpr int kCopyRows = 4;
+// written, take 83 us (6.5 TB/s; 4 rows a thread 93, 1 row 89).
+constexpr int kCopyRows = 2;
 template <int CH>
 __global__ void __launch_bounds__(256) paged_copy_kernel(PagedView c, PagedView to, int keep,
                                                          const int32_t *__restrict__ idx) {
@@ -193,8 +214,8 @@ __global__ void __launch_bounds__(256) paged_copy_kernel(PagedView c, PagedView 
 cudaError_t paged_append(const PagedView &c, const uint16_t *k, const uint16_t *v, int64_t k_row, int64_t k_head,
                          int64_t v_row, int64_t v_head, const int32_t *seq, const int32_t *slot, int rows,
                          cudaStream_t st) {
-  const int ch = c.hd / 8;
-  const int64_t blocks = (int64_t(rows) * c.kv_heads * ch + 255) / 256;
+  const int per = 256 / (c.hd / 8) * kAppendRows;
+  const int64_t blocks = (int64_t(rows) * c.kv_heads + per - 1) / per;
   if (c.hd == 128)
     paged_append_kernel<16><<<unsigned(blocks), 256, 0, st>>>(c, k, v, k_row, k_head, v_row, v_head, seq, slot, rows);
   else
