@@ -63,6 +63,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048;
+constexpr int kSelAhead = 8;      // weights a thread loads at once
 constexpr int kSelCache = 49152;  // keys a CTA can hold in shared memory (192 KB)
 
 // Exclusive prefix sum of v over the CTA's threads.
@@ -88,9 +89,10 @@ __device__ __forceinline__ int sel_scan(int v, int *warps) {
 // memory (a row of up to 49,152; longer ones are read again, from the L2 cache); then every thread counts what
 // stays of a run of candidates, and writes it behind what the threads before it count.
 //
-// Bound by the passes over a row by one SM, not by its bytes: 128 rows of up to 32,771 weights (10 MB) take 40 us, one
-// CTA an SM. Adding a warp's equal digits at once (ballots), or loading 4 or 8 keys ahead, was no faster, and rows of
-// one value are not slower without.
+// Bound by the passes over a row by one SM, not by its bytes: 128 rows of up to 32,771 weights (10 MB) take 20 us, one
+// CTA an SM; with one weight loaded at a time 29. Adding a warp's equal digits at once (ballots) or several copies of
+// the histogram were no faster, and rows of one value are not slower without. A CTA that also copied what it kept
+// took longer (136 us against 133 then): the SMs with few rows end early and HBM is not full.
 __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, int keep, int first, int recent, int cache,
                                                                    int32_t *__restrict__ idx,
                                                                    int32_t *__restrict__ to_lengths) {
@@ -121,16 +123,26 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     for (int d = tid; d < kSelBins; d += kSelThreads) hist[d] = 0;
     __syncthreads();
-    for (int j0 = 0; j0 < cand; j0 += kSelThreads) {
-      const int j = j0 + tid;
-      uint32_t key = 0;
-      if (j < cand) {
-        key = pass == 0 || !cached ? weight_key(w[j]) : sel_keys[j];
-        if (pass == 0 && cached) sel_keys[j] = key;
+    if (pass == 0 || !cached) {
+      for (int j0 = 0; j0 < cand; j0 += kSelAhead * kSelThreads) {
+        float x[kSelAhead];
+#pragma unroll
+        for (int u = 0; u < kSelAhead; ++u) x[u] = j0 + u * kSelThreads + tid < cand ? w[j0 + u * kSelThreads + tid] : 0.f;
+#pragma unroll
+        for (int u = 0; u < kSelAhead; ++u) {
+          const int j = j0 + u * kSelThreads + tid;
+          if (j >= cand) break;
+          const uint32_t key = weight_key(x[u]);
+          if (pass == 0 && cached) sel_keys[j] = key;
+          if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], 1);
+        }
       }
-      const bool in = j < cand && (key & known) == prefix;
-      const int digit = (key >> shift) & ((1 << bits) - 1);
-      if (in) atomicAdd(&hist[digit], 1);
+    } else {
+#pragma unroll 4
+      for (int j = tid; j < cand; j += kSelThreads) {
+        const uint32_t key = sel_keys[j];
+        if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], 1);
+      }
     }
     __syncthreads();
     // thread t holds bins 2 t and 2 t + 1 from the largest digit down
@@ -154,6 +166,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedView c, 
   const int run = ((cand + kSelThreads - 1) / kSelThreads) | 1;
   const int j0 = int(min(int64_t(cand), int64_t(tid) * run)), j1 = min(cand, j0 + run);
   int gt = 0, eq = 0;
+#pragma unroll 4
   for (int j = j0; j < j1; ++j) {
     const uint32_t key = cached ? sel_keys[j] : weight_key(w[j]);
     gt += key > prefix;
