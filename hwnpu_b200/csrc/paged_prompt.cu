@@ -872,55 +872,67 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
         tc_fence_after();
       }
       const int q = lane & 3;
-      uint16_t *out0 = p.a.o + int64_t(sg.row0 + tok0) * p.a.o_row + hq0 * p.a.o_head + 8 * q;
-      float *part0 = p.part_o + (int64_t(part) * p.slot_rows + x * p.tokens * rep) * HD + 2 * q;
 #pragma unroll 1
-      for (int u = 0; u < HD / 16; ++u) {
-        const int r16 = 16 * (u & 1), col = 32 * (u >> 1);
-        uint32_t o[16];
-        if (n > 0) {
-          pp_ldo(to + (uint32_t(r16) << 16) + col, o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = 0u;
-        }
-        if (u == HD / 16 - 1 && n > 0) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) tc_arrive(&ofree[x]);
-        }
+      for (int r16 = 0; r16 < 32; r16 += 16) {
+        // of the two rows whose pieces this lane handles: where they go, and what they are multiplied by
+        uint16_t *out[2];
+        float *unfinished[2];
+        float fr[2];
+        bool there[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const int lr = r16 + 8 * b + (lane >> 2), rr = 32 * (warp & 3) + lr;  // the row in the warp, in the tile
-          const float fr = __shfl_sync(0xffffffffu, f, lr);
           const int tt = token_of(rr);
+          fr[b] = __shfl_sync(0xffffffffu, f, lr);
+          there[b] = tt < left;
+          out[b] = p.a.o + int64_t(sg.row0 + tok0 + tt) * p.a.o_row + (hq0 + rr - tt * rep) * p.a.o_head + 8 * q;
+          unfinished[b] = p.part_o + (int64_t(part) * p.slot_rows + x * p.tokens * rep + rr) * HD + 2 * q;
+        }
+#pragma unroll 1
+        for (int col = 0; col < HD; col += 32) {
+          uint32_t o[16];
+          if (n > 0) {
+            pp_ldo(to + (uint32_t(r16) << 16) + col, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0u;
+          }
           if (part < 0) {
-            // words of column blocks i; the quad's 4 x 4 words are transposed: lane q gets block q
-            uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = pp_pack<BF>(__uint_as_float(o[4 * i + 2 * b]) * fr, __uint_as_float(o[4 * i + 2 * b + 1]) * fr);
+            for (int b = 0; b < 2; ++b) {
+              // words of column blocks i; the quad's 4 x 4 words are transposed: lane q gets block q
+              uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 1) ? w[i] : w[i + 1], 1);
-              if (q & 1) w[i] = got;
-              else w[i + 1] = got;
+              for (int i = 0; i < 4; ++i)
+                w[i] = pp_pack<BF>(__uint_as_float(o[4 * i + 2 * b]) * fr[b], __uint_as_float(o[4 * i + 2 * b + 1]) * fr[b]);
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 1) ? w[i] : w[i + 1], 1);
+                if (q & 1) w[i] = got;
+                else w[i + 1] = got;
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 2) ? w[i] : w[i + 2], 2);
+                if (q & 2) w[i] = got;
+                else w[i + 2] = got;
+              }
+              if (there[b]) *reinterpret_cast<uint4 *>(out[b] + col) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+          } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 2) ? w[i] : w[i + 2], 2);
-              if (q & 2) w[i] = got;
-              else w[i + 2] = got;
-            }
-            uint16_t *out = out0 + tt * p.a.o_row + (rr - tt * rep) * p.a.o_head + col;
-            if (tt < left) *reinterpret_cast<uint4 *>(out) = make_uint4(w[0], w[1], w[2], w[3]);
-          } else if (tt < left) {
-            float *out = part0 + int64_t(rr) * HD + col;
+            for (int b = 0; b < 2; ++b)
+              if (there[b])
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint2 *>(out + 8 * i) = make_uint2(o[4 * i + 2 * b], o[4 * i + 2 * b + 1]);
+                for (int i = 0; i < 4; ++i)
+                  *reinterpret_cast<uint2 *>(unfinished[b] + col + 8 * i) = make_uint2(o[4 * i + 2 * b], o[4 * i + 2 * b + 1]);
           }
         }
+      }
+      if (n > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc_arrive(&ofree[x]);
       }
       seg_done(k);
     }
