@@ -77,11 +77,16 @@ __device__ __forceinline__ int sel_scan(int v, int *warps) {
   }
   if (lane == 31) warps[warp] = x;
   __syncthreads();
-  int before = 0;
-#pragma unroll 4
-  for (int w = 0; w < kSelThreads / 32; ++w) before += w < warp ? warps[w] : 0;
+  static_assert(kSelThreads == 1024, "a lane a warp");
+  int upto = warps[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  const int before = __shfl_sync(0xffffffffu, upto, max(warp - 1, 0));
   __syncthreads();
-  return before + x - v;
+  return (warp > 0 ? before : 0) + x - v;
 }
 
 // One CTA a (sequence, kv head): the slots to keep into idx, ascending. The key of the last candidate that stays
