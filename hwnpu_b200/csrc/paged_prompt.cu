@@ -34,7 +34,7 @@
 // With head_dim 128 the halves of a tile are two chains (S, softmax, P V, the same half's next S), so that the softmax
 // has one half's scores while the tensor cores have the other's P. An MMA of 64 slots takes nearly as long as one
 // of 128 (59 clocks against 64), and it still pays: one chain a tile took 565 us for the 16,384-token prompt, two
-// take 533 (914 TFLOP/s; copies alone bound it at 403). With 64 there are two CTAs an SM instead.
+// 533 then. With 64 there are two CTAs an SM instead.
 // The next block's K, V, Q and first scores are under way while a block's last tile and output are.
 //
 // Arithmetic. S and O are float32. P = exp2(S scale log2(e) - m) is rounded to the cache's type (the MMA
@@ -42,6 +42,11 @@
 // than 2^8, which rescales O in tensor memory; P is at most 256 then, and fp16's P is held 2^7 higher
 // so that its smallest weights stand for 2^-32. (A polynomial for some of the exponentials, on the FMA
 // pipes, was slower: 617 us against 583 for the 16,384-token prompt with a quarter of them.)
+//
+// Measured. 16,384 tokens of 16 heads over 8 of 128, window 4,096: 521 us, 935 TFLOP/s (57% of a library GEMM's rate);
+// without the copies 506 then, without the MMAs 411, without both and the exponentials 300: no one part bounds it.
+// 512 tokens of 32 heads over 8 after 16,389: 154 us, 907 TFLOP/s, tensor pipe 50%, exponentials 50%. 16 ragged
+// prompts of up to 2,050 of 64 heads over 8 of 64, window 128: 176 us, 52% of the issue slots, tensor pipe 12%.
 //
 // Every mbarrier wait is bounded (about a second of SM clocks): one that runs out records a code that
 // hc_device_check reports and lets every other wait of the CTA return; the CTA still waits, bounded,
@@ -78,7 +83,7 @@ struct PpSmem {
   static constexpr int kTile = kHalves * kPpHalf;  // Q of a tile, or K or V of 128 slots
   // CTAs an SM: tensor memory has room for one with head_dim 128, and for two with 64 when a tile has one half's
   // scores at a time. Four tiles of one chain each then fill each other's gaps, a block's start and end among them:
-  // 186 us against 240 with two tiles of two chains for ragged prompts in a window of 128.
+  // 186 us against 240 with two tiles of two chains for ragged prompts in a window of 128, when both were measured.
   static constexpr int kCtas = HD == 128 ? 1 : 2;
   static constexpr int kBufs = HD == 128 ? 2 : 1;  // halves of S a tile
   static constexpr int kStages = HD == 128 ? 5 : 4;
@@ -395,8 +400,8 @@ __device__ __forceinline__ void pp_share(const PpArgs &p, PpShare *sh, long long
 
 template <int HD, bool BF>
 __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
-    paged_prompt_kernel(const PpArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                        const __grid_constant__ CUtensorMap qmap) {
+    paged_prompt_kernel(const PpArgs p, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap) {
   using Sm = PpSmem<HD>;
   constexpr int ST = Sm::kStages, NB = Sm::kBufs, CH = Sm::kHeld;
   constexpr int kCopy = kPpSoft / 32, kMma = kCopy + 1, kWalk = kCopy + 3;  // warps
@@ -753,7 +758,8 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
       // block's last row the latter, too
       const int pos = rt < left ? sg.p0 + tok0 + rt : -1;
       const bool windowed = p.a.window > 0;
-      const int wlo = windowed ? pos - p.a.window + 1 : -(1 << 30), wmax = windowed ? pmax - p.a.window + 1 : -(1 << 30);
+      const int wlo = windowed ? pos - p.a.window + 1 : -(1 << 30);
+      const int wmax = windowed ? pmax - p.a.window + 1 : -(1 << 30);
       const int ga = sg.ga, b0 = sg.b0 - sg.ga, groups = sg.groups;
       // groups [whole0, whole1) are seen by every row of the block: slots from wmax to pmin, in one run
       const int whole0 = max(b0 > 0 ? ga : 0, (max(wmax, 0) + kPpGroup - 1) / kPpGroup - b0);
@@ -1108,7 +1114,8 @@ cudaError_t paged_prompt(const PagedView &c, const PagedQuery &a, const int32_t 
   EncodeFn enc = pp_encoder();
   if (!enc) return cudaErrorNotSupported;
   PpMaps maps;
-  if (!pp_kv_map(enc, c, false, plan.box, &maps.k) || !pp_kv_map(enc, c, true, plan.box, &maps.v) || !pp_q_map(enc, c, a, rows, plan.tokens, &maps.q))
+  if (!pp_kv_map(enc, c, false, plan.box, &maps.k) || !pp_kv_map(enc, c, true, plan.box, &maps.v) ||
+      !pp_q_map(enc, c, a, rows, plan.tokens, &maps.q))
     return cudaErrorInvalidValue;
   uint8_t *base = static_cast<uint8_t *>(scratch);
   const PpArgs p{c, a, starts, rows, max_rows, plan.tokens, plan.blocks, plan.slot_rows, plan.box,

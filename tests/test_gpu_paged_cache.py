@@ -277,6 +277,33 @@ def test_prompt_large_scores():
     run_prompt(Case([2500], dtype=FP, mean=1.0), [300], scale=1e-6)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_prompt_maximum_that_moves_at_every_half_tile(hd, dtype):
+    # keys along one direction, 8 nats of score a 64 slots for a query of unit length along it, up or down: the running
+    # maximum is passed by more than 2^8 again and again, at the first and last half of tiles too. Scores stay
+    # below 300, so that a float32 score is off by less than 300 * 2^-22 < 1e-4 of a weight.
+    lens = [64, 65, 128, 129, 192, 193, 257, 330]
+    c = Case(lens, 8, 4, hd, 16, dtype)
+    u = c.randn(c.kv, hd)
+    for i, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        c.put(i, j, (j / 8.0).view(-1, 1, 1) * u + c.randn(n, c.kv, hd), c.randn(n, c.kv, hd))
+    run_prompt(c, lens)
+    run_prompt(c, [min(n, 70) for n in lens])
+
+
+@pytest.mark.parametrize("heads,kv,hd,dtype", [(8, 4, 128, BF), (16, 4, 64, FP), (10, 2, 128, FP), (4, 4, 64, BF)])
+@pytest.mark.parametrize("window", [0, 900])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_decode_of_few_sequences_is_split_and_joined(heads, kv, hd, dtype, window, sinks):
+    # few enough for one cluster a row; sequences of one group and of none among long ones
+    for accumulate in (False, True):
+        run_decode(Case([0, 7, 1500, 300, 2047], heads, kv, hd, 16, dtype), window, 5, sinks, accumulate)
+    if heads // kv <= 3:
+        run_prompt(Case([1500, 5, 300, 2047], heads, kv, hd, 32, dtype), [5, 3, 0, 1], window, 5, sinks)
+
+
 def test_prompt_and_decode_agree_on_one_row():
     c = Case([1, 77, 1500, 4001], 16, 8, 128, 16)
     q = c.queries(4)
