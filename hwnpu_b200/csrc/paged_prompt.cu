@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
   constexpr int kCopy = kPpSoft / 32, kMma = kCopy + 1, kWalk = kCopy + 3;  // warps
   extern __shared__ __align__(1024) uint8_t pp_sm[];  // the swizzle counts from 1,024-byte lines
   __shared__ uint64_t full[ST], empty[ST], vland, qfull, qempty, segfull[kPpSegs], segempty[kPpSegs];
-  __shared__ uint64_t sfull[2][2], pfull[2][2], ofull[2], ofree[2], done[2];
+  __shared__ uint64_t sfull[2][2], pfull[2][2], pvdone[2], ofull[2], ofree[2], done[2];
   __shared__ PpSeg segs[kPpSegs];
   __shared__ PpShare share;
   __shared__ long long sums[kPpThreads / 32];
@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
       tc_bar_init(&sfull[x][1], 1);
       tc_bar_init(&pfull[x][0], 4);
       tc_bar_init(&pfull[x][1], 4);
+      tc_bar_init(&pvdone[x], 1);
       tc_bar_init(&ofull[x], 1);
       tc_bar_init(&ofree[x], 4);
     }
@@ -716,8 +717,10 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
               if (half == 2 - NB) pp_wait(&full[s], turn, dead, 23);  // its first half
               scores(su, (half + NB) & 1, min(kPpHalfGroups, left - (NB - 1) * kPpHalfGroups));
             }
-            // with two halves of S, the last but one turn tells only (for a rescale) that P V of this half is done
-            tc_commit(u + 1 < nu ? &sfull[x][buf] : &ofull[x]);
+            // With two halves of S, the last but one turn brings no S and tells only (for a rescale) that P V of this
+            // half is done, on a barrier of its own: nothing makes the softmax wait for it, so on sfull the next block's
+            // first scores could complete a second phase before a slow softmax warp had looked at the first.
+            tc_commit(u + 1 == nu ? &ofull[x] : NB == 2 && u + 2 == nu ? &pvdone[x] : &sfull[x][buf]);
             if (half == 1 || u + 1 == nu) tc_commit(&empty[sv]);
             if (u + NB < nu && (((half + NB) & 1) == 1 || u + NB + 1 == nu)) tc_commit(&empty[su]);
             if (u + NB + 1 == nu) tc_commit(&qempty);
@@ -744,7 +747,7 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + x * 64 * NB + lanes, to = tmem + 128 * NB + x * HD + lanes;
     int done_blocks = 0;  // so far
-    uint32_t sph = 0;     // bit h: the parity of half h's next S
+    uint32_t sph = 0;     // bit h: the parity of half h's next S; bit 2: of pvdone's next turn, one a block of two halves or more
     for (int k = 0;; ++k) {
       const PpSeg &sg = seg_get(k);
       if (__any_sync(0xffffffffu, *dead || sg.h < 0)) break;
@@ -818,9 +821,10 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
           }
           if (u > 0) {
             // O has to be complete up to the last half: this S was issued behind its product, or with two of
-            // them the next half's S
+            // them the next half's S (behind the last half but one nothing: pvdone)
             if (NB == 2) {
-              pp_wait(&sfull[x][buf ^ 1], (sph >> (buf ^ 1)) & 1, dead, 30);
+              const bool end = u + 1 == nu;
+              pp_wait(end ? &pvdone[x] : &sfull[x][buf ^ 1], (sph >> (end ? 2 : buf ^ 1)) & 1, dead, 30);
               tc_fence_after();
             }
 #pragma unroll 1
@@ -858,10 +862,7 @@ __global__ void __launch_bounds__(kPpThreads, PpSmem<HD>::kCtas)
         const float2 lsum = pp_split(pp_add2(ls[0], ls[1]));
         l += lsum.x + lsum.y;
       }
-      if (NB == 2 && nu > 1) {  // the turn that no further S came with
-        pp_wait(&sfull[x][nu & 1], (sph >> (nu & 1)) & 1, dead, 24);
-        sph ^= 1u << (nu & 1);
-      }
+      if (NB == 2 && nu > 1) sph ^= 4u;
       // The rows: O / l, or what a second kernel makes it of. O is read as an MMA's fragment, 16 rows and 32
       // columns at a time, and a quad's words are transposed, so that rows leave in runs of 64 bytes.
       const int part = sg.part, hq0 = sg.h * rep;
