@@ -1,5 +1,6 @@
 """A long-context serving loop over PagedCache: prompts read in chunks, then decode steps that keep each
-sequence within a budget of cache rows a head, by evicting the rows that drew the least attention.
+sequence within a budget of cache rows a head, by evicting the rows that drew the least attention (of
+sliding layers, those behind the window).
 
     python examples/long_context.py [--seqs 8] [--prompt 3000] [--steps 400] [--budget 1024] [--check]
 
@@ -58,7 +59,7 @@ class Layer:
         cache.lengths.copy_(lengths)
         o = torch.empty_like(q)
         if starts is None:
-            # a sliding layer's slots keep their order but not their positions, so its window counts slots
+            # a sliding layer's newest slots are neighbours still, so its window counts slots
             cache.decode(q, o, DIM ** -0.5, window=self.window, first=FIRST, sinks=self.sinks,
                          accumulate=self.window == 0, scratch=self.scratch)
         else:
@@ -68,7 +69,9 @@ class Layer:
         return x * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + 1e-6).to(x.dtype)
 
     def evict(self, keep):
-        self.caches[0].evict(self.caches[1], keep, first=FIRST, recent=RECENT, scratch=self.scratch)
+        # a sliding layer sees its newest rows and the first ones, so it keeps those; the others choose by weight
+        recent = keep - FIRST if self.window else RECENT
+        self.caches[0].evict(self.caches[1], keep, first=FIRST, recent=recent, scratch=self.scratch)
         self.caches.reverse()
 
 
@@ -76,6 +79,8 @@ def run(seqs, prompt, steps, budget, layers=4, window=128, chunk=512, evicting=T
     """Returns (the last step's hidden rows, rows a head at the end, device milliseconds a decode step)."""
     gen = torch.Generator(device="cuda").manual_seed(seed)
     keep = budget * 3 // 4  # what an eviction leaves, so that it is not due every step
+    if evicting and keep < FIRST + max(window, RECENT):
+        raise ValueError(f"a budget of {budget} leaves {keep} rows, fewer than the first {FIRST} and a window of {window}")
     stack = [Layer(seqs, prompt + steps, max(keep, 1), window if n % 2 == 0 else 0, gen, dtype) for n in range(layers)]
     x_all = torch.randn((seqs, prompt, HEADS * DIM), device="cuda", generator=gen).to(dtype)
     ids = torch.arange(seqs, dtype=torch.int32, device="cuda")

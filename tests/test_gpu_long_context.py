@@ -82,3 +82,48 @@ def test_equals_plain_layers():
     # most 2^-8 of a value, with six of them a layer, summed as a walk and doubled for its tails
     err = float((got.float() - want).square().mean().sqrt())
     assert err < 2 * 2.0 ** -8 * (6 * 4 * 7) ** 0.5, err
+
+
+def rows_held(layer, seq, n):
+    """The marks (key column 0) of the rows sequence seq of a layer's cache holds, head by head."""
+    c = layer.caches[0]
+    slots = torch.arange(n, device="cuda")
+    return [c.k[c.block_table[seq].long()[slots // c.k.shape[2]], h, slots % c.k.shape[2], 0].tolist() for h in range(c.kv_heads)]
+
+
+@pytest.mark.parametrize("n,keep", [(300, 192), (300, 132), (1000, 300)])
+def test_sliding_layers_keep_their_window(n, keep):
+    import long_context as L
+
+    layer = L.Layer(2, n, keep, 128, torch.Generator(device="cuda").manual_seed(0), torch.float16)
+    c, slots = layer.caches[0], torch.arange(n, dtype=torch.int32, device="cuda")
+    rows = slots.half().view(-1, 1, 1).expand(n, L.KV, L.DIM).contiguous()  # whole numbers below 2,048: exact in fp16
+    for seq in range(2):
+        c.append(rows, rows, torch.full_like(slots, seq), slots)
+    c.lengths.fill_(n)
+    layer.evict(keep)
+    torch.cuda.synchronize()
+    assert layer.caches[0].lengths.tolist() == [keep] * 2
+    # all the model can see of it: the first rows and the window, here with the newest of what lies between
+    want = [float(j) for j in [*range(L.FIRST), *range(n - keep + L.FIRST, n)]]
+    for seq in range(2):
+        assert all(held == want for held in rows_held(layer, seq, keep))
+
+
+def test_sliding_layers_do_not_feel_the_evictions():
+    import long_context as L
+
+    # one sliding layer alone: what its mask shows is always held, so only the order of sums differs. fp16 rows of unit
+    # mean square, 20 tokens that feed one another, six roundings of 2^-11 each, summed as a walk and doubled
+    x, held, _ = L.run(3, 300, 20, 256, layers=1, dtype=torch.float16)
+    y, full, _ = L.run(3, 300, 20, 256, layers=1, dtype=torch.float16, evicting=False)
+    assert held < full
+    err = float((x - y).float().square().mean().sqrt())
+    assert err < 2 * 2.0 ** -11 * (6 * 20) ** 0.5, err
+
+
+def test_a_budget_below_the_window_is_refused():
+    import long_context as L
+
+    with pytest.raises(ValueError, match="window"):
+        L.run(1, 200, 2, 160)
