@@ -132,6 +132,10 @@ __device__ __forceinline__ float2 pd_unpack(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
+// The sum of P V and of what P's rounding left times V, but P V alone where it is not finite: the rounding may have
+// left 0 or less, and an infinite value's product with that would turn the infinity into NaN.
+__device__ __forceinline__ float pd_whole(float pv, float left) { return isfinite(pv) ? pv + left : pv; }
+
 // The slots that queries at slots qmin .. n - 1 see, as groups of 16: ga of them from slot 0 on, then those from
 // slot 16 b0 on; slot j of them is seen by one of the queries when j < n and (j >= lo or j < first).
 struct PdSpan {
@@ -403,7 +407,8 @@ __global__ void __launch_bounds__(kPdWarps * 32, PdRing<HD>::kCtas) paged_decode
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float2 v = MANY ? make_float2(o[t][2 * b], o[t][2 * b + 1]) : make_float2(o[t][0] + o[t][2], o[t][1] + o[t][3]);
+      const float2 v = MANY ? make_float2(o[t][2 * b], o[t][2 * b + 1])
+                            : make_float2(pd_whole(o[t][0], o[t][2]), pd_whole(o[t][1], o[t][3]));
       *reinterpret_cast<float2 *>(po + (warp * ROWS + gq + 8 * b) * HD + 8 * t + 2 * cq) = v;
     }
   }
