@@ -145,6 +145,7 @@ SIGNATURES = {
     "hc_paged_prompt_run": (_err, [_p, _p, _p, C.c_int32, C.c_int32, C.c_int32, _p, C.c_uint64, _p]),
     "hc_paged_prompt_scratch": (_err, [_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                        C.POINTER(C.c_uint64)]),
+    "hc_paged_check": (_err, []),
     "hc_paged_evict_run": (_err, [_p, _p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _p, _p, C.c_uint64, _p]),
     "hc_paged_evict_scratch": (_err, [_p, C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
 }

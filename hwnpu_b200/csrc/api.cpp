@@ -133,6 +133,7 @@ HC_API char *hc_set_fault(const char *spec) {
   if (point == "alloc") hc::g_fault_point = hc::kFaultAlloc;
   else if (point == "h2d") hc::g_fault_point = hc::kFaultH2D;
   else if (point == "step") hc::g_fault_point = hc::kFaultStep;
+  else if (point == "wait") hc::g_fault_point = hc::kFaultWait;
   else return hc::make_error("hc_set_fault: unknown point " + point);
   hc::g_fault_left = n;
   return nullptr;
@@ -205,10 +206,13 @@ HC_API char *hc_device_check(hc_device *d) {
   HC_TRY_CUDA(cudaSetDevice(d->ordinal));
   HC_TRY_CUDA(cudaDeviceSynchronize());
   const int code = hc::tc_status_take();
-  if (code) return hc::make_error("a tensor-core GEMV wait ran out (code " + std::to_string(code) + ")");
-  const int prompt = hc::paged_status_take();
-  if (prompt) return hc::make_error("a wait of the paged prompt attention ran out (code " + std::to_string(prompt) + ")");
-  return nullptr;
+  int prompt = 0;
+  HC_TRY_CUDA(hc::paged_status_take(&prompt));
+  std::string what;
+  if (code) what = "a tensor-core GEMV wait ran out (code " + std::to_string(code) + ")";
+  if (prompt)
+    what += (code ? "; " : "") + std::string("a wait of the paged prompt attention ran out (code ") + std::to_string(prompt) + ")";
+  return what.empty() ? nullptr : hc::make_error(what);
 }
 
 HC_API char *hc_buf_alloc(hc_device *d, uint64_t size, int kind, hc_buf **out) {

@@ -104,7 +104,7 @@ char *make_error(const std::string &msg);
   } while (0)
 
 // ---- host-side fault injection (hc_set_fault) ----------------------------------------------
-enum FaultPoint { kFaultAlloc = 0, kFaultH2D = 1, kFaultStep = 2 };
+enum FaultPoint { kFaultAlloc = 0, kFaultH2D = 1, kFaultStep = 2, kFaultWait = 3 };
 // True when the armed fault of this point fires on this call.
 bool fault_fires(FaultPoint p);
 // The armed device stall in milliseconds (hc_set_fault "stall:MS"), cleared by the call; 0: none.

@@ -194,6 +194,17 @@ HC_API char *hc_paged_prompt_run(const hc_paged_cache *cache, const hc_paged_att
   });
 }
 
+HC_API char *hc_paged_check(void) {
+  return guarded([&]() -> char * {
+    const char *who = "hc_paged_check";
+    int code = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = hc::paged_status_take(&code);
+    if (char *err = launched(who, e)) return err;
+    return code ? fail(who, "a wait of the paged prompt attention ran out (code " + std::to_string(code) + ")") : nullptr;
+  });
+}
+
 HC_API char *hc_paged_evict_scratch(const hc_paged_cache *cache, int32_t keep, int32_t max_len, uint64_t *bytes) {
   return guarded([&]() -> char * {
     const char *who = "hc_paged_evict_scratch";

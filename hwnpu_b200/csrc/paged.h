@@ -62,9 +62,9 @@ size_t paged_prompt_scratch(const PagedView &c, int heads, int window, int first
                             int sms);
 cudaError_t paged_prompt(const PagedView &c, const PagedQuery &a, const int32_t *starts, int rows, int max_rows,
                          int max_len, void *scratch, int sms, cudaStream_t st);
-// The code of the first wait of the prompt kernel that ran out on the current device since the last
+// *code: of the first wait of the prompt kernel that ran out on the current device since the last
 // call (0: none), cleared.
-int paged_status_take();
+cudaError_t paged_status_take(int *code);
 
 }  // namespace hc
 

@@ -1091,11 +1091,13 @@ cudaError_t pp_launch(const PpArgs &p, const PpPlan &plan, const PpMaps &m, cuda
 
 }  // namespace
 
-int paged_status_take() {
-  int v = 0, zero = 0;
-  if (cudaMemcpyFromSymbol(&v, pp_status_word, sizeof(int)) != cudaSuccess) return 0;
-  if (v) cudaMemcpyToSymbol(pp_status_word, &zero, sizeof(int));
-  return v;
+cudaError_t paged_status_take(int *code) {
+  const int zero = 0;
+  *code = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(code, pp_status_word, sizeof(int));
+  if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(pp_status_word, &zero, sizeof(int));
+  if (e == cudaSuccess && !*code && fault_fires(kFaultWait)) *code = 99;  // an injected one
+  return e;
 }
 
 size_t paged_prompt_scratch(const PagedView &c, int heads, int window, int first, int rows, int max_rows, int max_len,

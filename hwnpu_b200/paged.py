@@ -126,6 +126,13 @@ class PagedCache:
         A.check(A.lib().hc_paged_prompt_scratch(self._ref, heads, window, first, rows, max_rows, max_len, C.byref(n)))
         return n.value
 
+    @staticmethod
+    def check():
+        """Waits for the current device's work and raises HcError if a bounded wait inside a prompt call ran out since
+        the last check: that call's output is not to be trusted. Nothing else reports it, so a caller polls it
+        where a result matters more than its latency."""
+        A.check(A.lib().hc_paged_check())
+
     def evict(self, to, keep, first=0, recent=0, kept=None, max_len=0, scratch=None, stream=None):
         """Copies at most `keep` slots a head of every sequence into the pages of `to`, in slot order: the
         `first` first, the `recent` last and the heaviest between. Writes to.lengths, to.weights and

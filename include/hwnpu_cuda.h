@@ -305,7 +305,8 @@ HC_API char *hc_stats_get(hc_session *s, hc_stats *out);
 
 /* Fault injection for tests (the reference fakes its drivers instead, testdata/zemock):
  * "alloc:N" fails the N-th device allocation from now, "h2d:N" the N-th host-to-device copy,
- * "step:N" the N-th hc_step, each with an error string; "stall:MS" (MS <= 2000) makes the next
+ * "step:N" the N-th hc_step, each with an error string; "wait:N" makes the N-th check of the paged prompt
+ * attention's waits from now (hc_paged_check, hc_device_check) find one that ran out; "stall:MS" (MS <= 2000) makes the next
  * hc_step, hc_speculate or hc_generate first wait MS milliseconds on the device, so that a shorter
  * timeout_ms runs out (HC_STATE_TIMEOUT, the sequences poisoned until hc_seq_reset); "" clears.
  * Nothing faults or hangs on the GPU: the stall is a bounded wait on the global timer. */
@@ -483,6 +484,13 @@ HC_API char *hc_paged_prompt_run(const hc_paged_cache *c, const hc_paged_attn *a
                                  uint64_t scratch_bytes, void *stream);
 HC_API char *hc_paged_prompt_scratch(const hc_paged_cache *c, int32_t heads, int32_t window, int32_t first,
                                      int32_t rows, int32_t max_rows, int32_t max_len, uint64_t *bytes);
+
+/* Health of hc_paged_prompt_run on the current device, for callers without an hc_device: an error string when
+ * a bounded wait inside one of its launches (about a second each) ran out since the last check of either
+ * kind (hc_device_check reads the same record) -- the results of that launch are not to be trusted -- else
+ * NULL; clears the record. Waits for the device's queued work first, so not inside a stream capture. The
+ * other hc_paged_* kernels never wait. */
+HC_API char *hc_paged_check(void);
 
 /* Cuts every sequence to at most `keep` slots a head and copies them, in slot order, into the pages of
  * `to`: its first `first` slots, its last `recent`, and of those between the ones with the largest

@@ -158,3 +158,20 @@ def test_last_rows_agree_with_decode(heads, kv, hd, dtype):
              scratch=torch.zeros(max(16, a.decode_scratch(heads)), dtype=torch.uint8, device="cuda"))
     # two roundings of weights and results, each at most the type's unit of values below 4
     assert float((prompt(a, q, rows, 0.09)[last].double() - dec.double()).abs().max()) <= 2 * U[dtype] * 4
+
+
+def test_a_wait_that_ran_out_is_reported_without_a_device_handle(device):
+    c = Case([300], 16, 8, 64)
+    rows = [300]
+    q = c.queries(300)
+    out = prompt(c.cache(), q, rows)
+    hb.PagedCache.check()
+    check(c, q, out, rows)
+    A.check(A.lib().hc_set_fault(b"wait:1"))  # on the host: no wait on the GPU runs out
+    with pytest.raises(hb.HcError, match="prompt attention ran out"):
+        c.cache().check()
+    hb.PagedCache.check()  # cleared
+    A.check(A.lib().hc_set_fault(b"wait:1"))
+    with pytest.raises(hb.HcError, match="prompt attention ran out"):
+        A.check(A.lib().hc_device_check(device.h))
+    A.check(A.lib().hc_device_check(device.h))
