@@ -66,13 +66,15 @@ char *heads_ok(const char *who, const hc::PagedView &c, int heads, int window, i
   return nullptr;
 }
 
-char *query(const char *who, const hc::PagedView &c, const hc_paged_attn *a, int max_len, hc::PagedQuery *out) {
+char *query(const char *who, const hc::PagedView &c, const hc_paged_attn *a, int rows, int max_len, hc::PagedQuery *out) {
   if (!a) return fail(who, "NULL attention arguments");
   if (!a->q || !a->o) return fail(who, "NULL q or o");
   if (char *e = heads_ok(who, c, a->heads, a->window, a->first, max_len)) return e;
   if (!aligned16(a->q) || !aligned16(a->o)) return fail(who, "q and o must be 16-byte aligned");
   if (!good_stride(a->q_row) || !good_stride(a->q_head) || !good_stride(a->o_row) || !good_stride(a->o_head))
     return fail(who, "strides must be multiples of 8 elements, from 0 to 2^38");
+  if ((rows > 1 && a->o_row < c.hd) || (a->heads > 1 && a->o_head < c.hd))
+    return fail(who, "rows of o must not overlap: its strides are at least head_dim");
   if (!std::isfinite(a->scale)) return fail(who, "scale must be finite");
   *out = hc::PagedQuery{static_cast<const uint16_t *>(a->q), static_cast<uint16_t *>(a->o), a->q_row, a->q_head,
                         a->o_row, a->o_head, a->sinks, a->scale, a->heads, a->heads / c.kv_heads, a->window, a->first};
@@ -145,7 +147,7 @@ HC_API char *hc_paged_decode_run(const hc_paged_cache *cache, const hc_paged_att
     hc::PagedQuery a;
     int sms = 0;
     if (char *e = view(who, cache, &c)) return e;
-    if (char *e = query(who, c, attn, max_len, &a)) return e;
+    if (char *e = query(who, c, attn, c.seqs, max_len, &a)) return e;
     if (accumulate && !c.weights) return fail(who, "accumulate needs a cache with weights");
     if (char *e = multiprocessors(who, &sms)) return e;
     const int bound = bound_of(c, max_len);
@@ -184,7 +186,7 @@ HC_API char *hc_paged_prompt_run(const hc_paged_cache *cache, const hc_paged_att
     if (rows < 0 || max_rows < 0) return fail(who, "rows and max_rows must not be negative");
     if (rows == 0 || max_rows == 0) return nullptr;
     if (!starts) return fail(who, "NULL starts");
-    if (char *e = query(who, c, attn, max_len, &a)) return e;
+    if (char *e = query(who, c, attn, rows, max_len, &a)) return e;
     if (char *e = multiprocessors(who, &sms)) return e;
     const int bound = bound_of(c, max_len), most = max_rows < rows ? max_rows : rows;
     if (char *e = scratch_ok(who, scratch, scratch_bytes,

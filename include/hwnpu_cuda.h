@@ -447,7 +447,8 @@ typedef struct hc_paged_cache {
 typedef struct hc_paged_attn {
   const void *q;               /* [rows][heads][head_dim] of the cache's type, 16-byte aligned */
   void *o;                     /* [rows][heads][head_dim] of the cache's type, 16-byte aligned */
-  int64_t q_row, q_head, o_row, o_head; /* strides in elements, multiples of 8 */
+  int64_t q_row, q_head, o_row, o_head; /* strides in elements, multiples of 8; o's at least head_dim
+                                         * where there is more than one row (head) */
   const float *sinks;          /* [heads], or NULL */
   float scale;
   int32_t heads;               /* a multiple of kv_heads: query head h reads kv head

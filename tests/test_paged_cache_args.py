@@ -138,3 +138,10 @@ def test_python_checks():
                      (lambda: ok.evict(ok, 4, kept=torch.zeros(1, 2, 5, dtype=torch.int32)), "kept")):
         with pytest.raises(hb.HcError, match=why):
             bad()
+
+
+@pytest.mark.parametrize("kw", [dict(o_row=0), dict(o_head=0), dict(o_row=120), dict(o_head=64)])
+def test_an_output_that_overlaps_itself_is_refused(kw):
+    for call in calls(cache(), attn(**kw)):
+        with pytest.raises(hb.HcError, match="overlap"):
+            call()
