@@ -67,7 +67,7 @@ class PagedCacheDesc(C.Structure):
                 ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("row_stride", C.c_int64),
                 ("table_stride", C.c_int64), ("type", C.c_int32), ("seqs", C.c_int32), ("kv_heads", C.c_int32),
                 ("head_dim", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32), ("max_pages", C.c_int32),
-                ("pad_", C.c_int32)]
+                ("device", C.c_int32)]
 
 
 class PagedAttn(C.Structure):

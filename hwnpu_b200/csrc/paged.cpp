@@ -26,6 +26,10 @@ char *guarded(F f) {
 
 char *fail(const char *who, const std::string &what) { return hc::make_error(std::string(who) + ": " + what); }
 
+char *launched(const char *who, cudaError_t e) {
+  return e == cudaSuccess ? nullptr : fail(who, cudaGetErrorString(e));
+}
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // A stride the kernels' 16-byte loads and the tensor maps can take.
@@ -50,6 +54,13 @@ char *view(const char *who, const hc_paged_cache *c, hc::PagedView *out) {
     return fail(who, "strides must be multiples of 8 elements, from 0 to 2^38");
   if (c->row_stride < c->head_dim || (c->kv_heads > 1 && hs < c->head_dim) || (c->pages > 1 && ps < c->head_dim))
     return fail(who, "rows must not overlap: every stride is at least head_dim");
+  if (c->device) {
+    int current = 0;
+    if (char *e = launched(who, cudaGetDevice(&current))) return e;
+    if (current != c->device - 1)
+      return fail(who, "the cache is on device " + std::to_string(c->device - 1) + ", but device " +
+                           std::to_string(current) + " is current");
+  }
   int shift = 4;
   while ((1 << shift) < c->page_size) ++shift;
   *out = hc::PagedView{static_cast<uint16_t *>(c->k), static_cast<uint16_t *>(c->v), c->block_table, c->lengths,
@@ -86,10 +97,6 @@ char *scratch_ok(const char *who, const void *scratch, uint64_t have, uint64_t n
     return fail(who, "scratch of " + std::to_string(have) + " bytes, " + std::to_string(need) + " are needed");
   if (need && !aligned16(scratch)) return fail(who, "scratch must be 16-byte aligned");
   return nullptr;
-}
-
-char *launched(const char *who, cudaError_t e) {
-  return e == cudaSuccess ? nullptr : fail(who, cudaGetErrorString(e));
 }
 
 // Multiprocessors of the current device.

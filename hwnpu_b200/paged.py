@@ -2,10 +2,13 @@
 
 The cache and every operand are device tensors of the caller: objects with data_ptr(), shape, stride()
 and dtype, such as torch's. Nothing is allocated or copied; a call enqueues its kernels on `stream` (a
-cudaStream_t as an integer; None: the default stream) and returns. Wrong arguments raise HcError.
+cudaStream_t as an integer; None: the default stream) and returns. Wrong arguments raise HcError; torch's
+tensors among them when they are not on the cache's GPU, or that is not the current one (where other objects
+are is the caller's to know).
 """
 
 import ctypes as C
+import sys
 
 from . import _abi as A
 
@@ -40,14 +43,27 @@ class PagedCache:
         if weights is not None:
             _need(str(weights.dtype).endswith("float32") and tuple(weights.shape) == (seqs, heads, width * page)
                   and weights.is_contiguous(), "PagedCache: weights must be float32 [seqs][kv_heads][max_pages * page_size]")
+        torch = sys.modules.get("torch")
+        self._gpu = None  # the GPU of torch's tensors; -2, which no get_device() gives: they are elsewhere
+        if torch is not None and isinstance(k, torch.Tensor):
+            self._gpu = k.get_device() if k.is_cuda else -2
+            _need(all(t is None or t.device == k.device for t in (v, block_table, lengths, weights)),
+                  "PagedCache: the cache's tensors must be on one device")
         self.k, self.v, self.block_table, self.lengths, self.weights = k, v, block_table, lengths, weights
         self.seqs, self.kv_heads, self.head_dim, self.dtype = seqs, heads, dim, k.dtype
         self.desc = A.PagedCacheDesc(k.data_ptr(), v.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
                                      weights.data_ptr() if weights is not None else None, k.stride(0), k.stride(1),
                                      k.stride(2), block_table.stride(0), _TYPES[str(k.dtype)], seqs, heads, dim, page,
-                                     pages, width, 0)
+                                     pages, width, 0 if self._gpu is None or self._gpu < 0 else self._gpu + 1)
         self._ref = C.addressof(self.desc)
         self._int32 = block_table.dtype
+
+    def _misplaced(self, *operands):
+        """Raises if a kernel would see an address of the host or of another GPU than the cache's, which the library
+        holds against the current one. (The short calls test their own operands first: this costs 0.3 us.)"""
+        _need(self._gpu >= 0, "PagedCache: the cache must be on a GPU")
+        _need(all(t is None or t.get_device() == self._gpu for t in operands),
+              "PagedCache: every tensor must be on the cache's GPU")
 
     def _attn(self, q, out, scale, window, first, sinks):
         rows, heads, dim = q.shape
@@ -86,6 +102,9 @@ class PagedCache:
         for t in (seq, slot):
             if t.dtype != self._int32 or t.shape != (rows,) or not t.is_contiguous():
                 raise A.HcError("PagedCache.append: seq and slot must be int32 [rows]")
+        if self._gpu is not None and not (k.get_device() == v.get_device() == seq.get_device() == slot.get_device()
+                                          == self._gpu):
+            self._misplaced(k, v, seq, slot)
         A.check(A.lib().hc_paged_append_run(self._ref, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
                                             seq.data_ptr(), slot.data_ptr(), rows, stream))
 
@@ -98,6 +117,10 @@ class PagedCache:
         _need(len(q.shape) == 3 and q.shape[0] == self.seqs, "PagedCache.decode: q must be [seqs][heads][head_dim]")
         a = self._attn(q, out, scale, window, first, sinks)
         p, n = self._scratch(scratch)
+        if self._gpu is not None and not (q.get_device() == out.get_device() == self._gpu
+                                          and (sinks is None or sinks.get_device() == self._gpu)
+                                          and (scratch is None or scratch.get_device() == self._gpu)):
+            self._misplaced(q, out, sinks, scratch)
         A.check(A.lib().hc_paged_decode_run(self._ref, C.addressof(a), max_len, 1 if accumulate else 0, p, n, stream))
 
     def decode_scratch(self, heads, max_len=0, window=0, first=0, accumulate=False):
@@ -117,6 +140,8 @@ class PagedCache:
             raise A.HcError("PagedCache.prompt: starts must be int32 [seqs + 1]")
         a = self._attn(q, out, scale, window, first, sinks)
         p, n = self._scratch(scratch)
+        if self._gpu is not None:
+            self._misplaced(q, out, starts, sinks, scratch)
         A.check(A.lib().hc_paged_prompt_run(self._ref, C.addressof(a), starts.data_ptr(), q.shape[0], max_rows, max_len,
                                             p, n, stream))
 
@@ -142,6 +167,8 @@ class PagedCache:
             _need(kept.dtype == self._int32 and kept.shape == (self.seqs, self.kv_heads, keep) and kept.is_contiguous(),
                   "PagedCache.evict: kept must be int32 [seqs][kv_heads][keep]")
         p, n = self._scratch(scratch)
+        if self._gpu is not None:
+            self._misplaced(to.k, kept, scratch)
         A.check(A.lib().hc_paged_evict_run(self._ref, to._ref, keep, first, recent, max_len,
                                            kept.data_ptr() if kept is not None else None, p, n, stream))
 

@@ -433,7 +433,8 @@ typedef struct hc_paged_cache {
   int32_t page_size;           /* a power of two, 16..1024 */
   int32_t pages;               /* pages k and v hold */
   int32_t max_pages;           /* most pages of a sequence; max_pages * page_size < 2^30 */
-  int32_t pad_;
+  int32_t device;              /* 1 + the device all this memory is on: a call while another one is current is
+                                * refused. 0: not checked */
 } hc_paged_cache;
 
 /* The query side of an attention call. A query at slot p sees the slots j <= p with

@@ -145,3 +145,54 @@ def test_an_output_that_overlaps_itself_is_refused(kw):
     for call in calls(cache(), attn(**kw)):
         with pytest.raises(hb.HcError, match="overlap"):
             call()
+
+
+def test_tensors_that_are_not_on_the_gpu_are_refused():
+    torch = pytest.importorskip("torch")
+    bf = torch.bfloat16
+    k = torch.zeros((4, 2, 16, 64), dtype=bf)
+    t, n, w = torch.zeros((1, 3), dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 2, 48))
+    c = hb.PagedCache(k, k.clone(), t, n, weights=w)
+    to = hb.PagedCache(k.clone(), k.clone(), t.clone(), n.clone(), weights=w.clone())
+    q, new, starts = torch.zeros((1, 4, 64), dtype=bf), torch.zeros((1, 2, 64), dtype=bf), torch.zeros(2, dtype=torch.int32)
+    scratch = torch.zeros(1 << 16, dtype=torch.uint8)
+    for call in (lambda: c.decode(q, q.clone(), 1.0, scratch=scratch), lambda: c.append(new, new, n, n),
+                 lambda: c.prompt(q, q.clone(), starts, 1, 1.0, scratch=scratch), lambda: c.evict(to, 4, scratch=scratch)):
+        with pytest.raises(hb.HcError, match="on a GPU"):
+            call()
+    with pytest.raises(hb.HcError, match="one device"):
+        hb.PagedCache(k, torch.zeros((4, 2, 16, 64), dtype=bf, device="meta"), t, n)
+
+
+@pytest.mark.gpu
+def test_tensors_of_another_place_are_refused():
+    # refused by the binding: no kernel sees any of these addresses
+    torch = pytest.importorskip("torch")
+    bf, dev = torch.bfloat16, "cuda"
+    k = torch.zeros((4, 2, 16, 64), dtype=bf, device=dev)
+    t, n = torch.zeros((1, 3), dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    w = torch.zeros((1, 2, 48), device=dev)
+    c = hb.PagedCache(k, k.clone(), t, n, weights=w)
+    to = hb.PagedCache(k.clone(), k.clone(), t.clone(), n.clone(), weights=w.clone())
+    q, new, starts = torch.zeros((1, 4, 64), dtype=bf, device=dev), torch.zeros((1, 2, 64), dtype=bf, device=dev), n.new_tensor([0, 1])
+    sinks, scratch = torch.zeros(4, device=dev), torch.zeros(1 << 16, dtype=torch.uint8, device=dev)
+    kept = torch.zeros((1, 2, 4), dtype=torch.int32, device=dev)
+    calls = {"decode": (lambda q, out, sinks, scratch: c.decode(q, out, 1.0, sinks=sinks, scratch=scratch), [q, q.clone(), sinks, scratch]),
+             "prompt": (lambda q, out, starts, sinks, scratch: c.prompt(q, out, starts, 1, 1.0, sinks=sinks, scratch=scratch),
+                        [q, q.clone(), starts, sinks, scratch]),
+             "append": (c.append, [new, new.clone(), n - 1, n - 1]),
+             "evict": (lambda kept, scratch: c.evict(to, 4, kept=kept, scratch=scratch), [kept, scratch])}
+    for f, good in calls.values():
+        f(*good)
+        for i in range(len(good)):
+            with pytest.raises(hb.HcError, match="cache's GPU"):
+                f(*[x.cpu() if i == j else x for j, x in enumerate(good)])
+        for held in {c, to} if f is calls["evict"][0] else {c}:
+            held.desc.device = 2  # as if it were on another GPU than the current one
+            with pytest.raises(hb.HcError, match="device 0 is current"):
+                f(*good)
+            held.desc.device = 1
+    torch.cuda.synchronize()
+    for bad in ({"v": k.cpu()}, {"block_table": t.cpu()}, {"lengths": n.cpu()}, {"weights": w.cpu()}):
+        with pytest.raises(hb.HcError, match="one device"):
+            hb.PagedCache(**{**dict(k=k, v=k, block_table=t, lengths=n, weights=w), **bad})
