@@ -2,9 +2,9 @@
 
 The cache and every operand are device tensors of the caller: objects with data_ptr(), shape, stride()
 and dtype, such as torch's. Nothing is allocated or copied; a call enqueues its kernels on `stream` (a
-cudaStream_t as an integer; None: the default stream) and returns. Wrong arguments raise HcError; torch's
-tensors among them when they are not on the cache's GPU, or that is not the current one (where other objects
-are is the caller's to know).
+cudaStream_t as an integer; None: torch's current stream, or the default one for other objects than
+torch's tensors) and returns. Wrong arguments raise HcError, torch's tensors among them when they are not on
+the cache's GPU or that is not the current one (where other objects are is the caller's to know).
 """
 
 import ctypes as C
@@ -46,7 +46,11 @@ class PagedCache:
         torch = sys.modules.get("torch")
         self._gpu = None  # the GPU of torch's tensors; -2, which no get_device() gives: they are elsewhere
         if torch is not None and isinstance(k, torch.Tensor):
-            self._gpu = k.get_device() if k.is_cuda else -2
+            self._gpu = -2
+            if k.is_cuda:
+                self._gpu = k.get_device()
+                # the current stream in 0.06 us; torch.cuda.current_stream().cuda_stream takes 1.3 to 3
+                self._current = torch._C._cuda_getCurrentRawStream
             _need(all(t is None or t.device == k.device for t in (v, block_table, lengths, weights)),
                   "PagedCache: the cache's tensors must be on one device")
         self.k, self.v, self.block_table, self.lengths, self.weights = k, v, block_table, lengths, weights
@@ -105,6 +109,8 @@ class PagedCache:
         if self._gpu is not None and not (k.get_device() == v.get_device() == seq.get_device() == slot.get_device()
                                           == self._gpu):
             self._misplaced(k, v, seq, slot)
+        if stream is None and self._gpu is not None:
+            stream = self._current(self._gpu)
         A.check(A.lib().hc_paged_append_run(self._ref, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
                                             seq.data_ptr(), slot.data_ptr(), rows, stream))
 
@@ -121,6 +127,8 @@ class PagedCache:
                                           and (sinks is None or sinks.get_device() == self._gpu)
                                           and (scratch is None or scratch.get_device() == self._gpu)):
             self._misplaced(q, out, sinks, scratch)
+        if stream is None and self._gpu is not None:
+            stream = self._current(self._gpu)
         A.check(A.lib().hc_paged_decode_run(self._ref, C.addressof(a), max_len, 1 if accumulate else 0, p, n, stream))
 
     def decode_scratch(self, heads, max_len=0, window=0, first=0, accumulate=False):
@@ -142,6 +150,7 @@ class PagedCache:
         p, n = self._scratch(scratch)
         if self._gpu is not None:
             self._misplaced(q, out, starts, sinks, scratch)
+            stream = self._current(self._gpu) if stream is None else stream
         A.check(A.lib().hc_paged_prompt_run(self._ref, C.addressof(a), starts.data_ptr(), q.shape[0], max_rows, max_len,
                                             p, n, stream))
 
@@ -169,6 +178,7 @@ class PagedCache:
         p, n = self._scratch(scratch)
         if self._gpu is not None:
             self._misplaced(to.k, kept, scratch)
+            stream = self._current(self._gpu) if stream is None else stream
         A.check(A.lib().hc_paged_evict_run(self._ref, to._ref, keep, first, recent, max_len,
                                            kept.data_ptr() if kept is not None else None, p, n, stream))
 
