@@ -243,7 +243,8 @@ HC_API char *hc_paged_evict_run(const hc_paged_cache *cache, const hc_paged_cach
     if (keep > to.cap) return fail(who, "keep is above the capacity of the cache it copies into");
     if (c.lengths == to.lengths || c.table == to.table || c.weights == to.weights)
       return fail(who, "the cache it copies into needs a block table, lengths and weights of its own");
-    const uint64_t need = uint64_t(c.seqs) * c.kv_heads * keep * sizeof(int32_t);
+    // the kept slots are written to `kept` or, without it, to the scratch
+    const uint64_t need = kept ? 0 : uint64_t(c.seqs) * c.kv_heads * keep * sizeof(int32_t);
     if (char *e = scratch_ok(who, scratch, scratch_bytes, need)) return e;
     return launched(who, hc::paged_evict(c, to, keep, first, recent, bound_of(c, max_len),
                                          kept ? kept : static_cast<int32_t *>(scratch), static_cast<cudaStream_t>(stream)));

@@ -183,7 +183,7 @@ class PagedCache:
                                            kept.data_ptr() if kept is not None else None, p, n, stream))
 
     def evict_scratch(self, keep, max_len=0):
-        """Bytes of scratch evict needs with these arguments."""
+        """Bytes of scratch evict needs with these arguments and without `kept` (with it, none)."""
         n = C.c_uint64()
         A.check(A.lib().hc_paged_evict_scratch(self._ref, keep, max_len, C.byref(n)))
         return n.value

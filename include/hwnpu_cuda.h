@@ -502,7 +502,7 @@ HC_API char *hc_paged_check(void);
  * came from, -1 past the new length. `to` has the type, heads, head_dim and seqs of c, may share its
  * pools and page size or have others, and none of its pages may be one that c's sequences use: pages
  * that other sequences share stay as they are, and the caller frees the old ones. scratch:
- * hc_paged_evict_scratch bytes, as in hc_paged_decode_run. */
+ * hc_paged_evict_scratch bytes, as in hc_paged_decode_run; none with `kept`. */
 HC_API char *hc_paged_evict_run(const hc_paged_cache *c, const hc_paged_cache *to, int32_t keep, int32_t first,
                                 int32_t recent, int32_t max_len, int32_t *kept, void *scratch,
                                 uint64_t scratch_bytes, void *stream);

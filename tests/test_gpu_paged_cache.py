@@ -558,3 +558,16 @@ def test_a_loop_of_all_four():
                 at = kept[0, h].tolist()
                 rows[h] = [[rows[h][z][j] for j in at] for z in range(2)]
             cur, n = 1 - cur, keep
+
+
+def test_evict_needs_no_scratch_beside_kept():
+    c = Case([300, 40], 8, 4, 64)
+    kept = [torch.zeros((2, 4, 64), dtype=torch.int32, device="cuda") for _ in range(2)]
+    to = [Case([64, 64], 8, 4, 64, seed=9) for _ in range(2)]
+    a = c.cache()
+    a.evict(to[0].cache(), 64, recent=8, kept=kept[0], scratch=torch.zeros(a.evict_scratch(64), dtype=torch.uint8, device="cuda"))
+    a.evict(to[1].cache(), 64, recent=8, kept=kept[1])
+    torch.cuda.synchronize()
+    assert torch.equal(kept[0], kept[1]) and torch.equal(to[0].lengths, to[1].lengths)
+    with pytest.raises(hb.HcError, match="scratch"):
+        a.evict(to[1].cache(), 64, recent=8)
