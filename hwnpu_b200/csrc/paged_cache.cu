@@ -94,7 +94,7 @@ __device__ __forceinline__ int sel_scan(int v, int *warps) {
 // memory (a row of up to 49,152; longer ones are read again, from the L2 cache); then every thread counts what
 // stays of a run of candidates, and writes it behind what the threads before it count.
 //
-// Bound by the passes over a row by one SM, not by its bytes (70% of the issue slots): 128 rows of up to 32,771 weights
+// Bound by the passes over a row by one SM, not by its bytes (64% of the issue slots): 128 rows of up to 32,771 weights
 // (10 MB) take 20 us, one CTA an SM; with one weight loaded at a time 29. Adding a warp's equal digits at once (ballots) or several copies of
 // the histogram were no faster, and rows of one value are not slower without. A CTA that also copied what it kept
 // took longer (136 us against 133 then): the SMs with few rows end early and HBM is not full.

@@ -26,13 +26,15 @@
 //                at no further MMA; B is V by ldmatrix.trans. O is float32
 // Of several tokens both halves of A are rows, and the weights are rounded to the cache's type once.
 // The four warps' (m, l, O) are joined in shared memory, the splits' by a second kernel or, up to 8 of them,
-// by their cluster over distributed shared memory, all in a fixed order. With `accumulate` the scores are kept in scratch (float32) and the visible slots' weights
-// exp2(S - m) / l are summed over the heads once m and l are known.
+// by their cluster over distributed shared memory, all in a fixed order. With `accumulate` the scores are kept in scratch
+// (float32, room for the capacity: 4 bytes a slot and query head, so that a sequence past max_len is as fast; scores
+// computed over again there took 530 us against 221 for 64 sequences of up to 8,200 and a max_len of 4,000) and
+// the visible slots' weights exp2(S - m) / l are summed over the heads once m and l are known.
 //
-// Measured. One sequence of 131,071 slots (32 heads over 8 of 128): 90 us, 5.98 TB/s, 91% of the copy rate. 64 sequences
-// of up to 8,200 with their weights: 204 us, 5.37 TB/s. 128 in a window of 128 (64 heads over 8 of 64): 13 us,
-// 1,024 CTAs of three rounds in two waves; 5 rows each of 8 sequences of 500 to 2,100: 18 us, nine rounds and their
-// latencies. With 2 stages and more CTAs an SM: 14.1, 19.8.
+// Measured, on several GPUs. One sequence of 131,071 slots (32 heads over 8 of 128): 90 to 93 us, 5.8 to 6.0 TB/s, 88 to
+// 91% of the copy rate. 64 sequences of up to 8,200 with their weights: 203 to 208 us, 5.25 to 5.37 TB/s. 128 in a
+// window of 128 (64 heads over 8 of 64): 13 us, 1,024 CTAs of three rounds in two waves; 5 rows each of 8 sequences of
+// 500 to 2,100: 18 us, nine rounds and their latencies. With 2 stages and more CTAs an SM: 14.1, 19.8.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -43,10 +43,11 @@
 // so that its smallest weights stand for 2^-32. (A polynomial for some of the exponentials, on the FMA
 // pipes, was slower: 617 us against 583 for the 16,384-token prompt with a quarter of them.)
 //
-// Measured. 16,384 tokens of 16 heads over 8 of 128, window 4,096: 521 us, 935 TFLOP/s (57% of a library GEMM's rate);
-// without the copies 506 then, without the MMAs 411, without both and the exponentials 300: no one part bounds it.
-// 512 tokens of 32 heads over 8 after 16,389: 154 us, 907 TFLOP/s, tensor pipe 50%, exponentials 50%. 16 ragged
-// prompts of up to 2,050 of 64 heads over 8 of 64, window 128: 176 us, 52% of the issue slots, tensor pipe 12%.
+// Measured, on several GPUs. 16,384 tokens of 16 heads over 8 of 128, window 4,096: 525 to 537 us, 907 to 927 TFLOP/s
+// (56% of a library GEMM's rate); when it took 533, 506 without the copies, 411 without the MMAs, 300 without both and
+// the exponentials: no one part bounds it. 512 tokens of 32 heads over 8 after 16,389: 156 to 161 us, 870 to 898
+// TFLOP/s, tensor pipe 49%, exponentials 50%. 16 ragged prompts of up to 2,050 of 64 heads over 8 of 64, window 128:
+// 177 us, 52% of the issue slots, tensor pipe 12%.
 //
 // Every mbarrier wait is bounded (about a second of SM clocks): one that runs out records a code that
 // hc_device_check reports and lets every other wait of the CTA return; the CTA still waits, bounded,

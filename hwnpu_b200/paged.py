@@ -119,7 +119,7 @@ class PagedCache:
         """Attention of one new token a sequence: q, out [seqs][heads][head_dim], row i the token in slot
         lengths[i] - 1. It sees the last `window` slots (0: all) and the `first` first ones. With
         accumulate the visible slots' weights grow by what its heads gave them. scratch: device bytes
-        (decode_scratch)."""
+        (decode_scratch; with accumulate 4 a sequence, head and visible slot of the capacity)."""
         _need(len(q.shape) == 3 and q.shape[0] == self.seqs, "PagedCache.decode: q must be [seqs][heads][head_dim]")
         a = self._attn(q, out, scale, window, first, sinks)
         p, n = self._scratch(scratch)
@@ -169,7 +169,8 @@ class PagedCache:
 
     def evict(self, to, keep, first=0, recent=0, kept=None, max_len=0, scratch=None, stream=None):
         """Copies at most `keep` slots a head of every sequence into the pages of `to`, in slot order: the
-        `first` first, the `recent` last and the heaviest between. Writes to.lengths, to.weights and
+        `first` first, the `recent` last and the heaviest between. Only decode gathers weights: straight after a
+        prompt all are 0 and the oldest slots stay; a cache read through a window needs recent >= window. Writes to.lengths, to.weights and
         kept (int32 [seqs][kv_heads][keep], the slots they came from, -1 past the new length)."""
         _need(isinstance(to, PagedCache), "PagedCache.evict: `to` must be a PagedCache")
         if kept is not None:

@@ -444,7 +444,8 @@ typedef struct hc_paged_cache {
  * gptoss/build.go:256-285, without sinks that term is absent). A query that sees nothing writes
  * zeros. Slots that no query sees may hold anything, infinities and NaN included; in
  * hc_paged_prompt_run a value row that one query sees and another of the same call does not has to
- * be finite. */
+ * be finite. A visible infinite value comes out infinite while its weight does not round to 0 in the
+ * cache's type (fp16: 2^-32 of the largest), NaN then. */
 typedef struct hc_paged_attn {
   const void *q;               /* [rows][heads][head_dim] of the cache's type, 16-byte aligned */
   void *o;                     /* [rows][heads][head_dim] of the cache's type, 16-byte aligned */
@@ -471,7 +472,9 @@ HC_API char *hc_paged_append_run(const hc_paged_cache *c, const void *k, const v
  * caller's bound of the lengths, for the split alone (0: the capacity); a longer sequence is
  * still read whole. With accumulate != 0 the cache's weights of every visible slot grow by the sum of
  * w_j over the kv head's query heads. scratch: hc_paged_decode_scratch bytes, 16-byte aligned, its
- * contents arbitrary and not kept; calls that overlap in time need scratch of their own. */
+ * contents arbitrary and not kept; calls that overlap in time need scratch of their own. With accumulate it
+ * holds 4 bytes a sequence, query head and slot that could be seen in the capacity (of a window, about window
+ * + first of them), whatever max_len is. */
 HC_API char *hc_paged_decode_run(const hc_paged_cache *c, const hc_paged_attn *a, int32_t max_len,
                                  int32_t accumulate, void *scratch, uint64_t scratch_bytes, void *stream);
 HC_API char *hc_paged_decode_scratch(const hc_paged_cache *c, int32_t heads, int32_t window, int32_t first,
@@ -496,8 +499,9 @@ HC_API char *hc_paged_check(void);
 
 /* Cuts every sequence to at most `keep` slots a head and copies them, in slot order, into the pages of
  * `to`: its first `first` slots, its last `recent`, and of those between the ones with the largest
- * accumulated weights (of two equal ones the lower slot; NaN counts below every number). Sequences of
- * at most keep slots are copied whole. Each kv head keeps slots of its own. to->lengths and, when `to`
+ * accumulated weights (of two equal ones the lower slot; NaN counts below every number). Only decode calls
+ * gather weights: where none has run since the rows were appended all are 0, and the oldest slots stay. A cache
+ * read through a window keeps its window with recent >= window. Sequences of at most keep slots are copied whole. Each kv head keeps slots of its own. to->lengths and, when `to`
  * has them, to->weights are written; kept (int32 [seqs][kv_heads][keep], or NULL) gets the slots the rows
  * came from, -1 past the new length. `to` has the type, heads, head_dim and seqs of c, may share its
  * pools and page size or have others, and none of its pages may be one that c's sequences use: pages
